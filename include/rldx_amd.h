@@ -914,6 +914,129 @@ hipError_t rldx_rope_interleaved_f32(const float* xq, const int64_t* q_strides, 
                                      const int64_t* freqs_strides, hipStream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Attention over a stream of tokens: sliding window, and a 4-bit K/V cache */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Causal GQA attention with a sliding window and sinks, bf16 in / out, fp32
+ * scores, softmax and sums.  Query i of seq_q stands at p = seq_k - seq_q + i
+ * (a prompt: seq_q = seq_k; a chunk or a single token behind a past: seq_q <
+ * seq_k <= 2^30) and sees key j iff
+ *   j <= p  and  (j > p - window  or  j < sinks)  and  key_mask[b, j] != 0.
+ * o = softmax over the visible keys of (q . k scale), times V; a query that sees
+ * no key gets zeros.  A key that a query does not see has no influence on it,
+ * whatever its K and V rows hold.  Query head h reads KV head h / (Hq / Hkv).
+ *   q, o [B, seq_q, Hq, D], k, v [B, seq_k, Hkv, D]: strides {batch, seq, head}
+ *   (3 int64 each, multiples of 8; D contiguous, 64 or 128), 16-byte aligned.
+ *   key_mask: NULL, or fp32 [B, seq_k] (row stride key_mask_batch_stride, 0 =
+ *   one row for every sequence), 4-byte aligned.  window >= 1, sinks >= 0.
+ * workspace: >= rldx_window_attention_workspace_bytes(...) bytes, 16-byte
+ * aligned, caller-owned (0 bytes: may be NULL), used until the call's launches
+ * have run.  One launch, or two where few query rows split the keys.
+ *
+ * No counterpart in the reference: the backbone's causal prefill
+ *   (rldx/inference/backbone/llm/engine/kernels/fused_llm_attention.py:379-770)
+ *   for streams that outgrow one prompt.
+ */
+hipError_t rldx_window_attention_bf16(const void* q, const int64_t* q_strides, const void* k,
+                                      const int64_t* k_strides, const void* v, const int64_t* v_strides, void* o,
+                                      const int64_t* o_strides, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                      int64_t seq_q, int64_t seq_k, int64_t head_dim, int64_t window, int64_t sinks,
+                                      const float* key_mask, int64_t key_mask_batch_stride, float scale,
+                                      void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of the call above; -1 for sizes it refuses. */
+int64_t rldx_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
+                                              int64_t seq_k, int64_t head_dim, int64_t window, int64_t sinks);
+
+/*
+ * A paged K/V cache in 4 bits and the page table of a batch of sequences.
+ * Values are held in OCP MXFP4: blocks of 32 along head_dim, e2m1 elements (0,
+ * .5, 1, 1.5, 2, 3, 4, 6 with a sign) and one e8m0 scale (2^(byte - 127), 255 =
+ * NaN) per block; 17/32 byte per value.  A page holds page_tokens slots of every
+ * KV head, page_tokens / 32 tiles of 34 head_dim bytes per head (byte order:
+ * csrc/kv4_cache.h).  Slot s of sequence b is slot s % page_tokens of page
+ * page_table[b][s / page_tokens].  Page ids are read on the device: an id outside
+ * [0, num_pages) is a missing page, and so is a slot at or past table_pages *
+ * page_tokens.  Nothing is read or written through a missing page.
+ */
+typedef struct rldx_kv4_cache {
+  void* data;                /* pages, 16-byte aligned                                            */
+  int64_t num_pages;         /* < 2^31                                                            */
+  int64_t kv_heads;
+  int64_t head_dim;          /* 64 or 128                                                         */
+  int64_t page_tokens;       /* power of two, 32 .. 2^20                                          */
+  int64_t page_stride;       /* bytes, multiple of 16                                             */
+  int64_t head_stride;       /* bytes, multiple of 16, >= rldx_kv4_page_bytes(page_tokens, D)     */
+  const int32_t* page_table; /* [batch, table_pages], device memory                               */
+  int64_t table_pages;       /* table_pages * page_tokens <= 2^30                                 */
+  int64_t page_table_stride; /* elements                                                          */
+} rldx_kv4_cache_t;
+
+/* Bytes of one page of one KV head; -1 for an unsupported page_tokens or head_dim. */
+int64_t rldx_kv4_page_bytes(int64_t page_tokens, int64_t head_dim);
+
+/*
+ * HOST function (host pointers): codes (16 bytes, the even element in the low
+ * half) and scale byte of `blocks` blocks of 32 bf16 values, by the very element
+ * functions of the append kernel, so that the format can be checked on the CPU.
+ */
+int rldx_host_kv4_encode_bf16(const void* x, void* codes, void* scales, int64_t blocks);
+
+/*
+ * Writes rows k, v [batch, seq, kv_heads, D] bf16 (strides {batch, seq, head},
+ * multiples of 8 elements, D contiguous, 16-byte aligned) to the slots
+ * starts[b] + i, i < counts[b] (int32 device memory; counts NULL: all seq rows).
+ * Per block of 32: amax = f 2^p, 1 <= f < 2, scale 2^e with e = p - 2 (f < 1.75)
+ * or p - 1, within [-125, 125] (an all-zero block: -125); elements x / 2^e to
+ * the nearest, ties to the even code, larger ones to 6, signs kept.  A block with
+ * an infinity or a NaN reads back as NaN.  Slots below 0 and slots of missing
+ * pages are skipped.  Two rows of one call must not write the same slot.
+ * One launch, no workspace.
+ * No counterpart in the reference, which keeps no K/V between calls.
+ */
+hipError_t rldx_kv4_append_bf16(const rldx_kv4_cache_t* cache, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, const int32_t* starts,
+                                const int32_t* counts, int64_t batch, int64_t seq, hipStream_t stream);
+
+/*
+ * The values that the slots starts[b] .. starts[b] + seq - 1 hold, as bf16 rows
+ * k, v [batch, seq, kv_heads, D] (layout as above; exact); a slot below 0 or of a
+ * missing page gives NaN.  A slot that nobody has written gives whatever its
+ * bytes stand for.  One launch, no workspace.
+ * No counterpart in the reference.
+ */
+hipError_t rldx_kv4_read_bf16(const rldx_kv4_cache_t* cache, const int32_t* starts, void* k,
+                              const int64_t* k_strides, void* v, const int64_t* v_strides, int64_t batch,
+                              int64_t seq, hipStream_t stream);
+
+/*
+ * Attention of q [batch, seq_q, Hq, D] bf16 over the cache, o like q (strides
+ * {batch, seq, head}, multiples of 8, D contiguous, 16-byte aligned).  Query i
+ * of sequence b stands at slot p = starts[b] + i (its own K / V already appended)
+ * and sees slot j iff j <= p and (j > p - window or j < sinks).  Queries i >=
+ * counts[b] (counts may be NULL: none), and those below slot 0, see nothing and
+ * get zeros.  A query that sees a slot of a missing page gets NaN; pages whose
+ * slots no query sees are not touched (a sliding window may give them back).
+ * Slots that a query does not see have no influence on it, whatever they hold.
+ * The products are those of the exact bf16 values, fp32 scores, softmax and sums.
+ * workspace: >= rldx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ * caller-owned (0 bytes: may be NULL), used until the call's launches have run.
+ * One or two launches, which depend on the sizes alone: starts, counts and the
+ * page table may change between the replays of a captured call.
+ * No counterpart in the reference.
+ */
+hipError_t rldx_kv4_attention_bf16(const void* q, const int64_t* q_strides, const rldx_kv4_cache_t* cache,
+                                   const int32_t* starts, const int32_t* counts, void* o, const int64_t* o_strides,
+                                   int64_t batch, int64_t q_heads, int64_t seq_q, int64_t window, int64_t sinks,
+                                   float scale, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of the call above; -1 for sizes it refuses. */
+int64_t rldx_kv4_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q,
+                                           int64_t head_dim, int64_t page_tokens, int64_t table_pages,
+                                           int64_t window, int64_t sinks);
+
+/* ------------------------------------------------------------------------ */
 /* Measurement                                                              */
 /* ------------------------------------------------------------------------ */
 

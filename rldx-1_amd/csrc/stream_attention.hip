@@ -1,0 +1,780 @@
+// Attention over a stream of tokens: a sliding window with sinks over bf16 K/V rows
+// (rldx_window_attention_bf16) and over the 4-bit paged cache (rldx_kv4_attention_bf16).
+//
+//   o_i = sum_j p_ij v_j,  p_ij = softmax over the visible j of (q_i . k_j scale);
+//   j is visible to a query at p iff j <= p and (j > p - window or j < sinks).
+//
+// rows_attn_kernel: few query rows per KV head (single tokens, chunks).  The rows of a KV head's
+// whole group, (token, head) pairs in that order, are the 16 columns of S^T = K Q^T, so K and V
+// are read once for the group.  Per 32 keys a wave runs
+//   S^T  = K Q^T  two 16-key blocks, v_mfma_f32_16x16x32_bf16 over head_dim
+//   O^T += V^T P^T  one 32-key step for each of head_dim / 16 blocks of dimensions
+// and P^T goes from the S^T accumulators to the B operand without leaving its lane: lane group g
+// holds keys 4 g .. 4 g + 3 of both blocks, and the V^T operand takes its 32 keys in that order.
+// V rows are turned by v_perm on pairs of rows that the lane itself has loaded (8 keys by head_dim / 16
+// dimensions a lane), so nothing goes through LDS but the merge of the workgroup's 4 waves, which
+// walk tiles w, w + 4, ...  Where the rows leave most CUs idle, `splits` workgroups share
+// the tiles of a row block and merge_kernel adds up their partial states (fp32, as the softmax
+// reference, the sum and the unnormalised O).
+#include <algorithm>
+
+#include "kv4_cache.h"
+#include "rldx_amd.h"
+
+namespace rldx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kTile = kv4::kTile;
+constexpr int kWaves = 4;
+constexpr int kMaxSlots = 1 << 30;
+constexpr float kMoveRef = 3.f;  // log2 units: the softmax reference moves when a score exceeds it by 2^3
+
+struct StreamArgs {
+  const uint16_t* q;
+  int64_t q_sb, q_ss, q_sh;
+  uint16_t* o;
+  int64_t o_sb, o_ss, o_sh;
+  // bf16 rows
+  const uint16_t *k, *v;
+  int64_t k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;
+  const float* mask;  // [batch, sk] or null
+  int64_t mask_sb;
+  // 4-bit cache
+  const uint8_t* cache;
+  int64_t page_stride, head_stride;  // bytes
+  int num_pages, page_shift;
+  const int32_t* table;
+  int64_t table_sb;
+  const int32_t* starts;
+  const int32_t* counts;  // or null
+  int limit;              // readable keys: seq_k, or the slots of a row of the table
+  int batch, sq, hq, hkv, group, window, sinks;
+  int row_tiles, splits;
+  float scale_log2;
+  float* part;  // [batch hkv row_tiles splits][rows per tile][D] O, then the same rows' {reference, sum}
+};
+
+// The queries i0 .. i1 of a row block that see anything, and the tiles that hold what they see.
+struct Span {
+  int start;   // slot of query 0
+  int count;   // queries i >= count see nothing
+  int p0, p1;  // slots of the first and the last query of the block that sees anything, p1 < limit
+  int ns, w0;  // tiles [0, ns) hold the sinks, tiles from w0 (>= ns) on the window
+  int n;       // tiles in all
+};
+
+template <bool kCache>
+__device__ __forceinline__ Span span_of(const StreamArgs& a, int b, int row0, int rows) {
+  Span s;
+  s.count = a.sq;
+  if constexpr (kCache) {
+    s.start = min(max(a.starts[b], -kMaxSlots), kMaxSlots);
+    if (a.counts) s.count = min(s.count, a.counts[b]);
+  } else {
+    s.start = a.limit - a.sq;
+  }
+  const int i0 = max(row0 / a.group, -min(s.start, 0));
+  const int i1 = min((row0 + rows - 1) / a.group, s.count - 1);
+  s.p0 = s.start + i0;
+  s.p1 = min(s.start + i1, a.limit - 1);  // (a query past the limit is NaN whatever it sees)
+  if (i1 < i0 || s.p1 < s.p0) {
+    s.p0 = 0;
+    s.p1 = -1;
+    s.ns = s.w0 = s.n = 0;
+    return s;
+  }
+  s.ns = (min(a.sinks, s.p1 + 1) + kTile - 1) / kTile;
+  s.w0 = max(s.ns, max(0, s.p0 - a.window + 1) / kTile);
+  s.n = s.ns + max(0, s.p1 / kTile + 1 - s.w0);
+  return s;
+}
+
+// Splits that a row block of n tiles uses: none with less than one tile for each wave.
+__device__ __forceinline__ int splits_of(int splits, int n) { return max(1, min(splits, (n + kWaves - 1) / kWaves)); }
+
+// over the 4 lanes of a query (lanes l, l ^ 16, l ^ 32, l ^ 48): the swaps leave a lane's own value and its
+// partner's in the two registers
+__device__ __forceinline__ float quad_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
+}
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+
+// What a lane loads of a tile of 32 keys.
+template <int D, bool kCache>
+struct Raw;
+template <int D>
+struct Raw<D, true> {
+  u32x4 k[2];     // D = 64: two dwords of each
+  u32x4 v[2];     // D = 64: the first
+  uint32_t ks[2];
+  u32x2 vs;
+};
+template <int D>
+struct Raw<D, false> {
+  u32x4 k[2][D / 32];
+  u32x4 v[8];  // D = 64: two dwords of each
+  float m[2][4];
+};
+
+__device__ __forceinline__ bf16x8 dequant8(uint32_t c, float s) {
+  const u32x4 r = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {  // either half of a bf16 pair
+  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+}
+
+// NT: 16-row blocks of a workgroup.
+template <int D, int NT, bool kCache>
+__global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel(StreamArgs a) {
+  constexpr int RB = 16 * NT;
+  constexpr int KS = D / 32;   // MFMA steps over head_dim
+  constexpr int W = D / 16;    // dimensions of a lane's V columns, blocks of O^T
+  constexpr int OP = D + 4;    // pitch of O in LDS (floats)
+  constexpr int PF = kCache ? 2 : 1;  // tiles a wave has in flight
+  __shared__ __attribute__((aligned(16))) float sm_o[kWaves][16][OP];
+  __shared__ float sm_ml[kWaves][16][2];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int n16 = lane & 15, g = lane >> 4;
+
+  // work item: (batch, kv head, split, row tile)
+  int id = static_cast<int>(blockIdx.x);
+  const int rt = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int hk = id % a.hkv, b = id / a.hkv;
+
+  const int rows = a.sq * a.group;
+  const int row0 = rt * RB;
+  const Span sp = span_of<kCache>(a, b, row0, min(RB, rows - row0));
+  const int use = splits_of(a.splits, sp.n);
+  if (split >= use) return;
+  const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
+  const int t1 = static_cast<int>(static_cast<int64_t>(sp.n) * (split + 1) / use);
+  const int mine = t1 - t0 > wave ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;  // tiles t0 + wave + 4 it
+  auto tile_at = [&](int it) {
+    const int t = t0 + wave + kWaves * it;
+    return t < sp.ns ? t : sp.w0 + (t - sp.ns);
+  };
+
+  // this lane's queries: column n16 of each 16-row block
+  int pos[NT];      // slot, -1: sees nothing
+  bf16x8 qf[NT][KS];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = min(row0 + 16 * nt + n16, rows - 1);
+    const int i = r / a.group, h = hk * a.group + r - i * a.group;
+    pos[nt] = i < sp.count ? max(sp.start + i, -1) : -1;
+    const uint16_t* const src = a.q + b * a.q_sb + i * a.q_ss + h * a.q_sh + (kCache ? D / 4 : 8) * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      qf[nt][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + (kCache ? 8 : 32) * s));
+  }
+
+  // page ids of the wave's next 64 tiles, one a lane
+  int ids = -1, ids_base = 0;
+  auto load_ids = [&](int it0) {
+    ids_base = it0;
+    ids = -1;
+    if constexpr (kCache) {
+      const int it = it0 + lane;
+      if (it < mine) ids = a.table[b * a.table_sb + ((tile_at(it) * kTile) >> a.page_shift)];
+    }
+  };
+  load_ids(0);
+  auto page_of = [&](int it) {  // called with it ascending
+    if (it - ids_base >= 64) load_ids(it);
+    return __builtin_amdgcn_readlane(ids, it - ids_base);
+  };
+
+  auto load = [&](Raw<D, kCache>& raw, int it, int& page) {
+    const int k0 = tile_at(it) * kTile;
+    if constexpr (kCache) {
+      page = page_of(it);
+      if (page < 0 || page >= a.num_pages) {
+        page = -1;
+        raw = Raw<D, true>{};
+        return;
+      }
+      const uint8_t* const t = a.cache + page * a.page_stride + hk * a.head_stride +
+                               ((k0 & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int row = kt * 16 + n16;
+        if constexpr (D == 128) {
+          raw.k[kt] = *reinterpret_cast<const u32x4*>(t + row * 64 + g * 16);
+          raw.ks[kt] = t[32 * D + row * 4 + g];
+        } else {
+          const u32x2 c = *reinterpret_cast<const u32x2*>(t + row * 32 + g * 8);
+          raw.k[kt] = u32x4{c[0], c[1], 0, 0};
+          raw.ks[kt] = t[32 * D + row * 2 + (g >> 1)];
+        }
+      }
+      raw.v[0] = *reinterpret_cast<const u32x4*>(t + 16 * D + lane * (D / 4));
+      if constexpr (D == 128) raw.v[1] = *reinterpret_cast<const u32x4*>(t + 16 * D + lane * (D / 4) + 16);
+      raw.vs = *reinterpret_cast<const u32x2*>(t + 33 * D + ((n16 * W / 32) * 4 + g) * 8);
+    } else {
+      page = 0;
+      const int last = a.limit - 1;
+      const uint16_t* const kb = a.k + b * a.k_sb + hk * a.k_sh;
+      const uint16_t* const vb = a.v + b * a.v_sb + hk * a.v_sh + n16 * W;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const uint16_t* const src = kb + min(k0 + kt * 16 + n16, last) * a.k_ss + g * 8;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) raw.k[kt][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint16_t* const src = vb + min(k0 + (i >> 2) * 16 + g * 4 + (i & 3), last) * a.v_ss;
+        if constexpr (D == 128) {
+          raw.v[i] = *reinterpret_cast<const u32x4*>(src);
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+          raw.v[i] = u32x4{x[0], x[1], 0, 0};
+        }
+      }
+      if (a.mask) {
+        const float* const m = a.mask + b * a.mask_sb;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) raw.m[kt][r] = m[min(k0 + kt * 16 + g * 4 + r, last)];
+      }
+    }
+  };
+
+  floatx4 oacc[NT][W];
+  float m_ref[NT], l[NT];
+  bool poison[NT];  // a visible V block of this lane's dimensions is NaN, or the query stands past the limit
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) oacc[nt][j] = floatx4{0, 0, 0, 0};
+    m_ref[nt] = -__builtin_inff();
+    l[nt] = 0.f;
+    poison[nt] = pos[nt] >= a.limit;
+  }
+
+  // every query of the block sees something (the columns past the last row repeat it)
+  const bool all_rows = sp.p0 == sp.start + row0 / a.group && sp.p1 == sp.start + (min(row0 + RB, rows) - 1) / a.group;
+  auto visible = [&](int key, int p) { return key <= p && (key > p - a.window || key < a.sinks); };
+
+  auto compute = [&](Raw<D, kCache>& raw, int it, int page) {
+    const int k0 = tile_at(it) * kTile;
+    // every query of the block sees all 32 keys: no masks, and no key whose V may not be touched
+    bool full = page >= 0 && all_rows && k0 + kTile - 1 <= sp.p0 && (k0 > sp.p1 - a.window || k0 + kTile <= a.sinks);
+    if constexpr (!kCache) {
+      if (a.mask) {
+        bool any = false, all = true;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            any |= raw.m[kt][r] != 0.f;
+            all &= raw.m[kt][r] != 0.f;
+          }
+        if (!__any(any)) return;
+        full = full && __all(all);
+      }
+    }
+    // ---- S^T ----
+    floatx4 s[NT][2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][kt] = floatx4{0, 0, 0, 0};
+      float ks = 0.f;
+      if constexpr (kCache) ks = __builtin_bit_cast(float, raw.ks[kt] << 23);
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+        bf16x8 kf;
+        if constexpr (kCache) {
+          const uint32_t c = raw.k[kt][st];
+          kf = dequant8(c, ks);
+        } else {
+          kf = __builtin_bit_cast(bf16x8, raw.k[kt][st]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          s[nt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][st], s[nt][kt], 0, 0, 0);
+      }
+    }
+    // ---- visibility ----
+    bool odd_v = false;  // (wave-uniform) the tile's V holds something that is not finite: handled key by key
+    if (!full) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            bool ok = visible(k0 + kt * 16 + g * 4 + r, pos[nt]);
+            if constexpr (!kCache) ok = ok && (!a.mask || raw.m[kt][r] != 0.f);
+            const float sc = kCache && page < 0 ? __builtin_nanf("") : s[nt][kt][r];
+            s[nt][kt][r] = ok ? sc : -__builtin_inff();
+          }
+      if constexpr (kCache) {
+        bool dirty = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t e = (raw.vs[i >> 2] >> (8 * (i & 3))) & 255u;
+          dirty |= e >= 253;
+        }
+        odd_v = __any(dirty);
+      } else {
+        bool dirty = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < W / 2; ++j) dirty |= nonfinite2(raw.v[i][j]);
+        odd_v = __any(dirty);
+      }
+    }
+    // ---- softmax ----
+    bf16x8 pf[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float mt = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
+                       fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
+      mt *= a.scale_log2;
+      if (__any(mt > m_ref[nt] + kMoveRef)) {
+        const float nr = fmaxf(m_ref[nt], quad_max(mt));
+        const float al = m_ref[nt] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_ref[nt] - nr);
+        m_ref[nt] = nr;
+        l[nt] *= al;
+#pragma unroll
+        for (int j = 0; j < W; ++j) oacc[nt][j] *= al;
+      }
+      const float nm = m_ref[nt] == -__builtin_inff() ? 0.f : -m_ref[nt];
+      float ps = 0.f;
+      u32x4 pk;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          s[nt][kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][r], a.scale_log2, nm));
+          ps += s[nt][kt][r];
+        }
+        pk[2 * kt] = pack_bf16x2(s[nt][kt][0], s[nt][kt][1]);
+        pk[2 * kt + 1] = pack_bf16x2(s[nt][kt][2], s[nt][kt][3]);
+      }
+      l[nt] += ps;
+      pf[nt] = __builtin_bit_cast(bf16x8, pk);
+    }
+    // ---- V rows of the lane's 8 keys, W dimensions each, in bf16 pairs ----
+    uint32_t vr[8][W / 2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (kCache) {
+        const uint32_t e = (raw.vs[i >> 2] >> (8 * (i & 3))) & 255u;
+        const float sc = __builtin_bit_cast(float, e << 23);
+        if constexpr (D == 128) {
+          const uint32_t c = raw.v[i >> 2][i & 3];
+          vr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0));
+          vr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1));
+          vr[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2));
+          vr[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3));
+        } else {
+          const uint32_t c = raw.v[0][i >> 1];
+          if (i & 1) {
+            vr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2));
+            vr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3));
+          } else {
+            vr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0));
+            vr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1));
+          }
+        }
+        if (odd_v && e >= 253) {
+#pragma unroll
+          for (int j = 0; j < W / 2; ++j) vr[i][j] = 0;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) {
+          uint32_t w = raw.v[i][j];
+          if (odd_v) {
+            if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+            if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+          }
+          vr[i][j] = w;
+        }
+      }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      u32x4 vf;
+#pragma unroll
+      for (int tp = 0; tp < 4; ++tp)
+        vf[tp] = perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        oacc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf), pf[nt], oacc[nt][j], 0, 0, 0);
+    }
+    if (odd_v) {
+      // what the products above left out, for the queries that see it: this lane's dimensions are
+      // 4 W g .. 4 W g + 4 W - 1, O^T element (j, r) the one at W r + j among them
+      if constexpr (kCache) {
+        const uint8_t* const t = a.cache + page * a.page_stride + hk * a.head_stride +
+                                 ((k0 & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
+        for (int key = 0; page >= 0 && key < kTile; ++key) {
+          const uint32_t e = t[33 * D + (4 * W * g / 32 * 4 + kv4::v_group(key)) * 8 + kv4::v_unit(key)];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) poison[nt] = poison[nt] || (e >= 253 && visible(k0 + key, pos[nt]));
+        }
+      } else {
+        const uint16_t* const vb = a.v + b * a.v_sb + hk * a.v_sh + 4 * W * g;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int r4 = 0; r4 < 4; ++r4)
+            for (int gg = 0; gg < 4; ++gg) {
+              const int key = k0 + kt * 16 + gg * 4 + r4;
+              if (key >= a.limit || (a.mask && a.mask[b * a.mask_sb + key] == 0.f)) continue;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const float pr = __shfl(s[nt][kt][r4], n16 + 16 * gg);
+                if (!visible(key, pos[nt])) continue;
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                  for (int j = 0; j < W; ++j) {
+                    const uint16_t x = vb[key * a.v_ss + W * r + j];
+                    if ((x & 0x7f80) == 0x7f80) oacc[nt][j][r] += pr * bf16_bits_to_f32(x);
+                  }
+              }
+            }
+      }
+    }
+  };
+
+  Raw<D, kCache> raw[PF];
+  int page[PF];
+#pragma unroll
+  for (int u = 0; u < PF; ++u)
+    if (u < mine) load(raw[u], u, page[u]);
+  for (int it = 0; it < mine; it += PF) {
+#pragma unroll
+    for (int u = 0; u < PF; ++u) {
+      if (it + u >= mine) break;
+      Raw<D, kCache> cur = raw[u];
+      const int pg = page[u];
+      if (it + u + PF < mine) load(raw[u], it + u + PF, page[u]);
+      compute(cur, it + u, pg);
+    }
+  }
+
+  // ---- merge the 4 waves, one 16-row block after the other ----
+  const int tid = static_cast<int>(threadIdx.x);
+  const int mr = tid >> 4, md = (tid & 15) * W;  // the row and the first of W dimensions that this thread finishes
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float lsum = quad_sum(l[nt]);
+    if (nt) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < W; j += 4) {
+        floatx4 x = {oacc[nt][j][r], oacc[nt][j + 1][r], oacc[nt][j + 2][r], oacc[nt][j + 3][r]};
+        if (poison[nt]) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        *reinterpret_cast<floatx4*>(&sm_o[wave][n16][4 * W * g + W * r + j]) = x;
+      }
+    if (g == 0) {
+      sm_ml[wave][n16][0] = m_ref[nt];
+      sm_ml[wave][n16][1] = lsum;
+    }
+    __syncthreads();
+    const int row = row0 + 16 * nt + mr;
+    if (row < rows) {
+      float m = -__builtin_inff(), lt = 0.f, w[kWaves];
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        w[i] = sm_ml[i][mr][0] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm_ml[i][mr][0] - m);
+        lt = __builtin_fmaf(sm_ml[i][mr][1], w[i], lt);
+      }
+      float acc[W];
+#pragma unroll
+      for (int j = 0; j < W; j += 4) {
+        floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) x += *reinterpret_cast<const floatx4*>(&sm_o[i][mr][md + j]) * w[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j + e] = x[e];
+      }
+      const int i = row / a.group, h = hk * a.group + row - i * a.group;
+      if (a.splits == 1) {
+        const float inv = lt > 0.f ? 1.f / lt : lt == 0.f ? 1.f : lt;  // (nothing seen: O is 0, or NaN; lt NaN stays)
+        uint32_t out[W / 2];
+#pragma unroll
+        for (int j = 0; j < W; j += 2) out[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+        uint16_t* const dst = a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + md;
+        if constexpr (W == 8)
+          *reinterpret_cast<u32x4*>(dst) = u32x4{out[0], out[1], out[2], out[3]};
+        else
+          *reinterpret_cast<u32x2*>(dst) = u32x2{out[0], out[1]};
+      } else {
+        const int64_t item = (((static_cast<int64_t>(b) * a.hkv + hk) * a.row_tiles + rt) * a.splits + split) * RB + 16 * nt + mr;
+        const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * RB;
+#pragma unroll
+        for (int j = 0; j < W; j += 4)
+          *reinterpret_cast<floatx4*>(a.part + item * D + md + j) = floatx4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
+        if (md == 0) {
+          a.part[items * D + item * 2] = m;
+          a.part[items * D + item * 2 + 1] = lt;
+        }
+      }
+    }
+  }
+}
+
+// O of a query row from the partial states of its splits: wave w adds up splits w, w + 4, ...
+template <int D, bool kCache>
+__global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb) {
+  constexpr int E = D / 64;  // dimensions per lane
+  __shared__ float sm[kWaves][D];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int rows = a.sq * a.group;
+  int id = static_cast<int>(blockIdx.x);
+  const int row = id % rows;
+  id /= rows;  // b hkv + hk
+  const int b = id / a.hkv, hk = id - b * a.hkv;
+  const int rt = row / rb;
+  const Span sp = span_of<kCache>(a, b, rt * rb, min(rb, rows - rt * rb));
+  const int use = splits_of(a.splits, sp.n);  // <= 64
+  const int64_t first = (static_cast<int64_t>(id) * a.row_tiles + rt) * a.splits * rb + (row - rt * rb);
+  const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * rb;
+  float m = -__builtin_inff(), l = 0.f;
+  if (lane < use) {
+    const float* const ml = a.part + items * D + (first + static_cast<int64_t>(lane) * rb) * 2;
+    m = ml[0];
+    l = ml[1];
+  }
+  float top = m;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+  const float w = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+  l *= w;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+  float acc[E] = {};
+  for (int s0 = wave; s0 < use; s0 += 8 * kWaves) {
+    float x[8][E];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = min(s0 + u * kWaves, use - 1);
+      const float* const src = a.part + (first + static_cast<int64_t>(s) * rb) * D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[u][e] = src[e];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + u * kWaves >= use) break;
+      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s0 + u * kWaves));
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(x[u][e], ws, acc[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sm[wave][lane * E + e] = acc[e];
+  __syncthreads();
+  const int d = static_cast<int>(threadIdx.x);
+  if (d >= D / 2) return;
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 1.f : l;
+  float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    x0 += sm[i][2 * d];
+    x1 += sm[i][2 * d + 1];
+  }
+  const int i = row / a.group, h = hk * a.group + row - i * a.group;
+  *reinterpret_cast<uint32_t*>(a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + 2 * d) = pack_bf16x2(x0 * inv, x1 * inv);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// How a call is cut up; depends on sizes alone.
+struct Plan {
+  int nt, row_tiles, splits;
+  int64_t items;  // row blocks times splits
+  int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * 16 * nt * (head_dim + 2) * 4 : 0; }
+};
+
+// limit: readable keys.  false: sizes that the kernels do not take.
+bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t limit, int64_t head_dim,
+             int64_t window, int64_t sinks) {
+  if ((head_dim != 64 && head_dim != 128) || batch < 0 || q_heads < 0 || kv_heads <= 0 || q_heads % kv_heads ||
+      seq_q < 0 || limit < 0 || limit > kMaxSlots || window < 1 || sinks < 0 || batch > 65535 || q_heads > 65535)
+    return false;
+  const int64_t group = q_heads / kv_heads, rows = seq_q * group;
+  if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
+  p.nt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int64_t rb = 16 * p.nt;
+  p.row_tiles = static_cast<int>(rows == 0 ? 1 : (rows + rb - 1) / rb);
+  const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * p.row_tiles);
+  // tiles of the longest row block
+  const int64_t span = std::min(limit, std::min(window, limit) + rb / std::max<int64_t>(1, group) + 1);
+  const int64_t tiles = std::min((limit + kTile - 1) / kTile,
+                                 (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
+  const int64_t want = std::max<int64_t>(1, (p.nt == 4 ? 256 : 512) / blocks);
+  p.splits = static_cast<int>(std::min<int64_t>({64, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
+  p.items = blocks * p.splits;
+  return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
+}
+
+bool strides_ok(const int64_t* s) { return s && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }
+
+void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* o, const int64_t* os, int64_t batch,
+          int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t limit, int64_t window, int64_t sinks, float scale,
+          void* workspace) {
+  a = StreamArgs{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_sb = qs[0], a.q_ss = qs[1], a.q_sh = qs[2];
+  a.o = static_cast<uint16_t*>(o);
+  a.o_sb = os[0], a.o_ss = os[1], a.o_sh = os[2];
+  a.limit = static_cast<int>(limit);
+  a.batch = static_cast<int>(batch);
+  a.sq = static_cast<int>(seq_q);
+  a.hq = static_cast<int>(q_heads);
+  a.hkv = static_cast<int>(kv_heads);
+  a.group = static_cast<int>(q_heads / kv_heads);
+  a.window = static_cast<int>(std::min<int64_t>(window, kMaxSlots));
+  a.sinks = static_cast<int>(std::min<int64_t>(sinks, kMaxSlots));
+  a.row_tiles = p.row_tiles;
+  a.splits = p.splits;
+  a.scale_log2 = scale * kLog2e;
+  a.part = static_cast<float*>(workspace);
+}
+
+template <int D, bool kCache>
+hipError_t launch_rows(const StreamArgs& a, const Plan& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.items)), block(64 * kWaves);
+  if (p.nt == 1)
+    hipLaunchKernelGGL((rows_attn_kernel<D, 1, kCache>), grid, block, 0, stream, a);
+  else if (p.nt == 2)
+    hipLaunchKernelGGL((rows_attn_kernel<D, 2, kCache>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((rows_attn_kernel<D, 4, kCache>), grid, block, 0, stream, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.splits == 1) return e;
+  hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>(a.batch * a.hq * a.sq)), block, 0, stream, a,
+                     16 * p.nt);
+  return hipGetLastError();
+}
+
+// (scale 0 or below, infinite or NaN is refused)
+bool common_ok(const void* q, const int64_t* qs, const void* o, const int64_t* os, float scale) {
+  return strides_ok(qs) && strides_ok(os) && scale > 0.f && scale < __builtin_inff() && a16(q) && a16(o);
+}
+
+}  // namespace
+}  // namespace rldx
+
+using namespace rldx;
+
+extern "C" int64_t rldx_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                         int64_t seq_q, int64_t seq_k, int64_t head_dim,
+                                                         int64_t window, int64_t sinks) {
+  Plan p;
+  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks)) return -1;
+  return p.workspace(head_dim);
+}
+
+extern "C" hipError_t rldx_window_attention_bf16(const void* q, const int64_t* q_strides, const void* k,
+                                                 const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                                 void* o, const int64_t* o_strides, int64_t batch, int64_t q_heads,
+                                                 int64_t kv_heads, int64_t seq_q, int64_t seq_k, int64_t head_dim,
+                                                 int64_t window, int64_t sinks, const float* key_mask,
+                                                 int64_t key_mask_batch_stride, float scale, void* workspace,
+                                                 int64_t workspace_bytes, hipStream_t stream) {
+  Plan p;
+  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks) ||
+      !common_ok(q, q_strides, o, o_strides, scale) || !strides_ok(k_strides) || !strides_ok(v_strides) || !a16(k) ||
+      !a16(v) || reinterpret_cast<uintptr_t>(key_mask) % 4)
+    return hipErrorInvalidValue;
+  if (batch == 0 || q_heads == 0 || seq_q == 0) return hipSuccess;
+  if (!q || !k || !v || !o) return hipErrorInvalidValue;
+  if (p.workspace(head_dim) > 0 && (!workspace || !a16(workspace) || workspace_bytes < p.workspace(head_dim)))
+    return hipErrorInvalidValue;
+  StreamArgs a;
+  fill(a, p, q, q_strides, o, o_strides, batch, q_heads, kv_heads, seq_q, seq_k, window, sinks, scale, workspace);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.k_sb = k_strides[0], a.k_ss = k_strides[1], a.k_sh = k_strides[2];
+  a.v_sb = v_strides[0], a.v_ss = v_strides[1], a.v_sh = v_strides[2];
+  a.mask = key_mask;
+  a.mask_sb = key_mask_batch_stride;
+  return head_dim == 128 ? launch_rows<128, false>(a, p, stream) : launch_rows<64, false>(a, p, stream);
+}
+
+extern "C" int64_t rldx_kv4_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                      int64_t seq_q, int64_t head_dim, int64_t page_tokens,
+                                                      int64_t table_pages, int64_t window, int64_t sinks) {
+  Plan p;
+  if (rldx_kv4_page_bytes(page_tokens, head_dim) < 0 || table_pages < 0 || table_pages > kMaxSlots / page_tokens ||
+      !plan_of(p, batch, q_heads, kv_heads, seq_q, table_pages * page_tokens, head_dim, window, sinks))
+    return -1;
+  return p.workspace(head_dim);
+}
+
+extern "C" hipError_t rldx_kv4_attention_bf16(const void* q, const int64_t* q_strides, const rldx_kv4_cache_t* cache,
+                                              const int32_t* starts, const int32_t* counts, void* o,
+                                              const int64_t* o_strides, int64_t batch, int64_t q_heads, int64_t seq_q,
+                                              int64_t window, int64_t sinks, float scale, void* workspace,
+                                              int64_t workspace_bytes, hipStream_t stream) {
+  Plan p;
+  if (!kv4_cache_ok(cache) || !common_ok(q, q_strides, o, o_strides, scale) ||
+      !plan_of(p, batch, q_heads, cache->kv_heads, seq_q, cache->table_pages * cache->page_tokens, cache->head_dim,
+               window, sinks))
+    return hipErrorInvalidValue;
+  if (batch == 0 || q_heads == 0 || seq_q == 0) return hipSuccess;
+  if (!q || !o || !starts) return hipErrorInvalidValue;
+  if (p.workspace(cache->head_dim) > 0 &&
+      (!workspace || !a16(workspace) || workspace_bytes < p.workspace(cache->head_dim)))
+    return hipErrorInvalidValue;
+  StreamArgs a;
+  fill(a, p, q, q_strides, o, o_strides, batch, q_heads, cache->kv_heads, seq_q,
+       cache->table_pages * cache->page_tokens, window, sinks, scale, workspace);
+  a.cache = static_cast<const uint8_t*>(cache->data);
+  a.page_stride = cache->page_stride;
+  a.head_stride = cache->head_stride;
+  a.num_pages = static_cast<int>(cache->num_pages);
+  a.page_shift = __builtin_ctzll(static_cast<unsigned long long>(cache->page_tokens));
+  a.table = cache->page_table;
+  a.table_sb = cache->page_table_stride;
+  a.starts = starts;
+  a.counts = counts;
+  return cache->head_dim == 128 ? launch_rows<128, true>(a, p, stream) : launch_rows<64, true>(a, p, stream);
+}

@@ -287,6 +287,161 @@ Tensor ss3(const Tensor& x, const Tensor& p, const Tensor& qx, const Tensor& kx,
 }
 
 // ---------------------------------------------------------------------------
+// A stream of tokens: window attention, 4-bit K/V cache
+// ---------------------------------------------------------------------------
+// Strides {batch, seq, head} of bf16 rows [B, S, H, D]; false: not a form that is taken here.
+bool rows4(const Tensor& t, int64_t (&st)[3]) {
+  if (!bf16(t) || t.dim() != 4 || t.stride(3) != 1 || t.numel() == 0 ||
+      reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0)
+    return false;
+  for (int i = 0; i < 3; ++i) {
+    st[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    if (st[i] % 8 != 0) return false;
+  }
+  return true;
+}
+constexpr int64_t kNoWindow = int64_t{1} << 30;
+float softmax_scale(const std::optional<double>& scale, int64_t D) {
+  return static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(D)));
+}
+// (nothing allocated for a call that needs no workspace)
+Tensor workspace(const Tensor& t, int64_t n) {
+  return n > 0 ? at::empty({n}, t.options().dtype(at::kByte)) : Tensor();
+}
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+RLDX_OP(Window, "rldx_amd::window_attention");
+Tensor window_attention(const Tensor& q, const Tensor& k, const Tensor& v, SymInt window_, SymInt sinks_,
+                        const OptTensor& mask, std::optional<double> scale) {
+  const int64_t window = window_.guard_int(__FILE__, __LINE__), sinks = sinks_.guard_int(__FILE__, __LINE__);
+  int64_t qs[3], ks[3], vs[3];
+  if (rows4(q, qs) && rows4(k, ks) && rows4(v, vs) && one_device(q, k, v) && v.sizes() == k.sizes() &&
+      k.size(0) == q.size(0) && k.size(3) == q.size(3)) {
+    const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2), D = q.size(3), Sk = k.size(1), Hk = k.size(2);
+    const float* mp = nullptr;
+    int64_t ms = 0;
+    bool ok = true;
+    if (mask.has_value()) {
+      const Tensor& m = *mask;
+      ok = one_device(q, m) && m.scalar_type() == at::kFloat && (m.dim() == 1 || (m.dim() == 2 && (m.size(0) == 1 || m.size(0) == B))) &&
+           m.size(-1) == Sk && m.stride(-1) == 1;
+      if (ok) {
+        mp = m.data_ptr<float>();
+        ms = m.dim() == 2 && m.size(0) > 1 ? m.stride(0) : 0;
+      }
+    }
+    if (ok) {
+      const c10::OptionalDeviceGuard guard(q.device());
+      const int64_t need = rldx_window_attention_workspace_bytes(B, H, Hk, Sq, Sk, D, window, sinks);
+      if (need >= 0) {
+        Tensor out = at::empty(q.sizes(), q.options()), ws = workspace(q, need);
+        const int64_t os[3] = {Sq * H * D, H * D, D};
+        if (rldx_window_attention_bf16(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os, B, H, Hk,
+                                       Sq, Sk, D, window, sinks, mp, ms, softmax_scale(scale, D), ptr(ws), need,
+                                       stream_of(q)) == hipSuccess)
+          return out;
+      }
+    }
+  }
+  return python<Window, Tensor, const Tensor&, const Tensor&, const Tensor&, SymInt, SymInt, const OptTensor&,
+                std::optional<double>>(q, k, v, window_, sinks_, mask, scale);
+}
+
+// A cache of head_dim D with the tables of B sequences; false: not a form that is taken here.
+bool kv4(const Tensor& cache, const Tensor& table, const Tensor& starts, const OptTensor& counts, int64_t B, int64_t D,
+         rldx_kv4_cache_t& c) {
+  const auto ints = [&](const Tensor& t) { return one_device(cache, t) && t.scalar_type() == at::kInt; };
+  if (!cache.is_cuda() || cache.scalar_type() != at::kByte || cache.dim() != 3 || cache.numel() == 0 ||
+      cache.stride(2) != 1 || !(D == 64 || D == 128) || cache.size(2) % (34 * D) != 0 || !ints(table) ||
+      table.dim() != 2 || table.size(0) != B || table.stride(1) != 1 || !ints(starts) || starts.dim() != 1 ||
+      starts.size(0) != B || !starts.is_contiguous())
+    return false;
+  if (counts.has_value() &&
+      (!ints(*counts) || counts->dim() != 1 || counts->size(0) != B || !counts->is_contiguous()))
+    return false;
+  c = rldx_kv4_cache_t{cache.data_ptr(), cache.size(0), cache.size(1), D, cache.size(2) / (34 * D) * 32,
+                       cache.size(0) > 1 ? cache.stride(0) : cache.size(2),
+                       cache.size(1) > 1 ? cache.stride(1) : cache.size(2), table.data_ptr<int32_t>(), table.size(1),
+                       table.stride(0)};
+  return c.page_stride >= cache.size(2) && c.head_stride >= cache.size(2);
+}
+const int32_t* counts_ptr(const OptTensor& c) { return c.has_value() ? c->data_ptr<int32_t>() : nullptr; }
+
+RLDX_OP(Kv4Append, "rldx_amd::kv4_append");
+void kv4_append(const Tensor& cache, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& starts,
+                const OptTensor& counts) {
+  int64_t ks[3], vs[3];
+  rldx_kv4_cache_t c;
+  if (rows4(k, ks) && rows4(v, vs) && one_device(cache, k, v) && k.sizes() == v.sizes() &&
+      kv4(cache, table, starts, counts, k.size(0), k.size(3), c) && c.kv_heads == k.size(2)) {
+    const c10::OptionalDeviceGuard guard(k.device());
+    if (rldx_kv4_append_bf16(&c, k.data_ptr(), ks, v.data_ptr(), vs, starts.data_ptr<int32_t>(), counts_ptr(counts),
+                             k.size(0), k.size(1), stream_of(k)) == hipSuccess)
+      return;
+  }
+  python<Kv4Append, void, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&>(
+      cache, k, v, table, starts, counts);
+}
+// Autograd of the operator that writes: without a gradient in play the version of the cache is counted up here, not
+// in the Python kernel that stands between (8 us).
+void kv4_append_autograd(c10::DispatchKeySet ks, const Tensor& cache, const Tensor& k, const Tensor& v,
+                         const Tensor& table, const Tensor& starts, const OptTensor& counts) {
+  using Sig = void(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&);
+  static auto op = handle<Sig>(Kv4Append::name);
+  if (needs_autograd(cache) || needs_autograd(k) || needs_autograd(v) || cache.is_inference()) {
+    Autograd<Kv4Append, Sig>::call(ks, cache, k, v, table, starts, counts);
+    return;
+  }
+  op.redispatch(ks & c10::after_ADInplaceOrView_keyset, cache, k, v, table, starts, counts);
+  cache.unsafeGetTensorImpl()->bump_version();
+}
+
+using Two = std::tuple<Tensor, Tensor>;
+RLDX_OP(Kv4Read, "rldx_amd::kv4_read");
+Two kv4_read(const Tensor& cache, const Tensor& table, const Tensor& starts, SymInt count_, SymInt d_) {
+  const int64_t n = count_.guard_int(__FILE__, __LINE__), D = d_.guard_int(__FILE__, __LINE__);
+  rldx_kv4_cache_t c;
+  if (n > 0 && starts.dim() == 1 && starts.size(0) > 0 &&
+      kv4(cache, table, starts, std::nullopt, starts.size(0), D, c)) {
+    const c10::OptionalDeviceGuard guard(cache.device());
+    const int64_t B = starts.size(0), H = c.kv_heads, st[3] = {n * H * D, H * D, D};
+    Tensor k = at::empty({B, n, H, D}, cache.options().dtype(at::kBFloat16)), v = at::empty({B, n, H, D}, k.options());
+    if (rldx_kv4_read_bf16(&c, starts.data_ptr<int32_t>(), k.data_ptr(), st, v.data_ptr(), st, B, n, stream_of(k)) ==
+        hipSuccess)
+      return {k, v};
+  }
+  return python<Kv4Read, Two, const Tensor&, const Tensor&, const Tensor&, SymInt, SymInt>(cache, table, starts, count_,
+                                                                                           d_);
+}
+
+RLDX_OP(Kv4Attention, "rldx_amd::kv4_attention");
+Tensor kv4_attention(const Tensor& q, const Tensor& cache, const Tensor& table, const Tensor& starts,
+                     const OptTensor& counts, std::optional<SymInt> window_, SymInt sinks_,
+                     std::optional<double> scale) {
+  const int64_t sinks = sinks_.guard_int(__FILE__, __LINE__);
+  const int64_t window = window_.has_value() ? window_->guard_int(__FILE__, __LINE__) : kNoWindow;
+  int64_t qs[3];
+  rldx_kv4_cache_t c;
+  if (rows4(q, qs) && one_device(q, cache) && kv4(cache, table, starts, counts, q.size(0), q.size(3), c)) {
+    const int64_t B = q.size(0), Sq = q.size(1), H = q.size(2), D = q.size(3);
+    const c10::OptionalDeviceGuard guard(q.device());
+    const int64_t need =
+        rldx_kv4_attention_workspace_bytes(B, H, c.kv_heads, Sq, D, c.page_tokens, c.table_pages, window, sinks);
+    if (need >= 0) {
+      Tensor out = at::empty(q.sizes(), q.options()), ws = workspace(q, need);
+      const int64_t os[3] = {Sq * H * D, H * D, D};
+      if (rldx_kv4_attention_bf16(q.data_ptr(), qs, &c, starts.data_ptr<int32_t>(), counts_ptr(counts), out.data_ptr(),
+                                  os, B, H, Sq, window, sinks, softmax_scale(scale, D), ptr(ws), need,
+                                  stream_of(q)) == hipSuccess)
+        return out;
+    }
+  }
+  return python<Kv4Attention, Tensor, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                std::optional<SymInt>, SymInt, std::optional<double>>(q, cache, table, starts, counts, window_, sinks_,
+                                                                      scale);
+}
+
+// ---------------------------------------------------------------------------
 // SwiGLU, fused MLP, residual + norm
 // ---------------------------------------------------------------------------
 RLDX_OP(Swiglu, "rldx_amd::swiglu");
@@ -440,7 +595,6 @@ Tensor mlp(const Tensor& x, const Tensor& w, const Tensor& bias, SymInt split_) 
   return python<Mlp, Tensor, const Tensor&, const Tensor&, const Tensor&, SymInt>(x, w, bias, split_);
 }
 
-using Two = std::tuple<Tensor, Tensor>;
 // new = hidden + residual [+ deepstack]; normed = RMSNorm(new): outputs shaped like hidden, or undefined
 Two add_rmsnorm(const Tensor& h, const Tensor& r, const Tensor* ds, const Tensor& w) {
   if (bf16(h) && bf16(r) && (!ds || bf16(*ds)) && h.dim() >= 1 && h.numel() > 0 && one_device(h, r, w) &&
@@ -495,6 +649,12 @@ constexpr auto autograd_of(R (*)(A...)) { return &Autograd<Tag, R(A...)>::call; 
   X(M, "fused_attention_3way", Ss3, ss3); \
   X(M, "fused_mlp_swiglu", Mlp, mlp)
 
+#define RLDX_AMD(X, M)                              \
+  X(M, "swiglu", Swiglu, swiglu);                   \
+  X(M, "window_attention", Window, window_attention); \
+  X(M, "kv4_read", Kv4Read, kv4_read);              \
+  X(M, "kv4_attention", Kv4Attention, kv4_attention)
+
 TORCH_LIBRARY_IMPL(rldx_backbone, CUDA, m) { RLDX_BACKBONE(RLDX_IMPL, m); }
 TORCH_LIBRARY_IMPL(rldx_backbone, AutogradCUDA, m) { RLDX_BACKBONE(RLDX_AUTOGRAD, m); }
 TORCH_LIBRARY_IMPL(mem, CUDA, m) { RLDX_MEM(RLDX_IMPL, m); }
@@ -503,8 +663,14 @@ TORCH_LIBRARY_IMPL(ds, CUDA, m) { RLDX_DS(RLDX_IMPL, m); }
 TORCH_LIBRARY_IMPL(ds, AutogradCUDA, m) { RLDX_DS(RLDX_AUTOGRAD, m); }
 TORCH_LIBRARY_IMPL(ss, CUDA, m) { RLDX_SS(RLDX_IMPL, m); }
 TORCH_LIBRARY_IMPL(ss, AutogradCUDA, m) { RLDX_SS(RLDX_AUTOGRAD, m); }
-TORCH_LIBRARY_IMPL(rldx_amd, CUDA, m) { RLDX_IMPL(m, "swiglu", Swiglu, swiglu); }
-TORCH_LIBRARY_IMPL(rldx_amd, AutogradCUDA, m) { RLDX_AUTOGRAD(m, "swiglu", Swiglu, swiglu); }
+TORCH_LIBRARY_IMPL(rldx_amd, CUDA, m) {
+  RLDX_AMD(RLDX_IMPL, m);
+  RLDX_IMPL(m, "kv4_append", Kv4Append, kv4_append);
+}
+TORCH_LIBRARY_IMPL(rldx_amd, AutogradCUDA, m) {
+  RLDX_AMD(RLDX_AUTOGRAD, m);
+  m.impl("kv4_append", &kv4_append_autograd);
+}
 
 TORCH_LIBRARY(rldx_native, m) {
   m.def("remember_packed(Tensor w, Tensor packed) -> ()", &remember_packed);

@@ -64,6 +64,14 @@ class MsatStream(ctypes.Structure):
     ]
 
 
+class Kv4Cache(ctypes.Structure):
+    """rldx_kv4_cache_t"""
+
+    _fields_ = [("data", c_vp)] + [(n, c_i64) for n in ("num_pages", "kv_heads", "head_dim", "page_tokens", "page_stride",
+                                                        "head_stride")] + [
+        ("page_table", c_vp), ("table_pages", c_i64), ("page_table_stride", c_i64)]
+
+
 # name -> (restype, argtypes); must stay in sync with include/rldx_amd.h
 SIGNATURES = {
     "rldx_read_probe_sink_words": (c_i64, []),
@@ -177,6 +185,16 @@ SIGNATURES = {
                                            c_i64, c_i64, c_vp, c_i64p, c_vp]),
     "rldx_rope_interleaved_f32": (c_i32, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_i64,
                                           c_i64, c_i64, c_vp, c_i64p, c_vp]),
+    "rldx_window_attention_bf16": (c_i32, [c_vp, c_i64p] * 4 + [c_i64] * 8 + [c_vp, c_i64, c_f32, c_vp, c_i64, c_vp]),
+    "rldx_window_attention_workspace_bytes": (c_i64, [c_i64] * 8),
+    "rldx_kv4_page_bytes": (c_i64, [c_i64, c_i64]),
+    "rldx_host_kv4_encode_bf16": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i64]),
+    "rldx_kv4_append_bf16": (c_i32, [ctypes.POINTER(Kv4Cache), c_vp, c_i64p, c_vp, c_i64p, c_vp, c_vp, c_i64, c_i64,
+                                     c_vp]),
+    "rldx_kv4_read_bf16": (c_i32, [ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_vp]),
+    "rldx_kv4_attention_bf16": (c_i32, [c_vp, c_i64p, ctypes.POINTER(Kv4Cache), c_vp, c_vp, c_vp, c_i64p]
+                                + [c_i64] * 5 + [c_f32, c_vp, c_i64, c_vp]),
+    "rldx_kv4_attention_workspace_bytes": (c_i64, [c_i64] * 9),
 }
 
 ROPE_SIN_SIGNED = 1  # RLDX_ROPE_SIN_SIGNED

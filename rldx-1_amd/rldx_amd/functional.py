@@ -560,6 +560,171 @@ def llm_fused_attention(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: tor
     return out
 
 
+# ---------------------------------------------------------------------------
+# attention over a stream of tokens: sliding window, 4-bit K/V cache
+# ---------------------------------------------------------------------------
+NO_WINDOW = 1 << 30  # a window that holds every slot there can be
+
+
+def _rows4(t: torch.Tensor, what: str):
+    """Strides {batch, seq, head} of a bf16 [B, S, H, D] (0 for a dimension of one: it is never stepped over)."""
+    _require(t.dtype == BF16 and t.dim() == 4, f"{what} must be bf16 [B, S, H, D]")
+    _require(t.shape[3] in (64, 128) and t.stride(3) == 1, f"{what}: head_dim must be 64 or 128, contiguous")
+    st = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+    _require(all(s % 8 == 0 for s in st) and (t.data_ptr() % 16 == 0 or t.numel() == 0),
+             f"{what}: rows must be 16-byte aligned (strides multiples of 8)")
+    return _lib.i64_array(st)
+
+
+def _out4(q: torch.Tensor, out: Optional[torch.Tensor]):
+    if out is None:
+        return torch.empty(q.shape, dtype=BF16, device=q.device)
+    _require(out.shape == q.shape and all(out.shape[i] <= 1 or out.stride(i) != 0 for i in range(3)),
+             "out must match q, without overlapping rows")
+    return out
+
+
+def _softmax_scale(scale: Optional[float], D: int) -> float:
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    _require(0.0 < scale < math.inf, "scale must be positive and finite")
+    return scale
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                     key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None, *,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal GQA attention with a sliding window and sinks: q [B, Sq, Hq, D], k / v [B, Sk, Hkv, D] bf16 (any strides
+    with D contiguous and rows 16-byte aligned, D 64 or 128) -> [B, Sq, Hq, D].
+
+    Query i stands at p = Sk - Sq + i (Sq = Sk: a prompt; Sq < Sk: a chunk or a single token behind a past) and sees
+    key j iff j <= p, j > p - window or j < sinks, and key_mask[b, j] != 0 (fp32 [Sk] or [B or 1, Sk], optional: the
+    padding of a batch).  A query that sees no key gets zeros; keys that it does not see have no influence on it,
+    whatever they hold.  scale defaults to 1/sqrt(D) (rldx_window_attention_bf16)."""
+    _on_gpu(q, k, v, key_mask, out)
+    qs, ks, vs = _rows4(q, "q"), _rows4(k, "k"), _rows4(v, "v")
+    B, Sq, Hq, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    _require(k.shape[0] == B and k.shape[3] == D and v.shape == k.shape, "k and v must be [B, Sk, Hkv, D] matching q")
+    _require(Hkv > 0 and Hq % Hkv == 0, "q heads must be a multiple of kv heads")
+    _require(Sq <= Sk, "the queries are the last of the keys: Sq <= Sk")
+    window, sinks = int(window), int(sinks)
+    _require(window >= 1 and sinks >= 0, "window must be at least 1, sinks at least 0")
+    mp, ms = None, 0
+    if key_mask is not None:
+        _require(key_mask.dtype == F32 and key_mask.dim() in (1, 2) and key_mask.shape[-1] == Sk and
+                 (key_mask.stride(-1) == 1 or Sk <= 1) and (key_mask.dim() == 1 or key_mask.shape[0] in (1, B)),
+                 "key_mask must be fp32 [Sk] or [B or 1, Sk] with contiguous keys")
+        mp, ms = key_mask.data_ptr(), key_mask.stride(0) if key_mask.dim() == 2 and key_mask.shape[0] > 1 else 0
+    scale = _softmax_scale(scale, D)
+    out = _out4(q, out)
+    os_ = _rows4(out, "out")
+    if out.numel() == 0:
+        return out
+    lib = _lib.load()
+    need = int(lib.rldx_window_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sinks))
+    _require(need >= 0, "window_attention: sizes out of range (Sk and Sq * Hq / Hkv up to 2^30)")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(lib.rldx_window_attention_bf16(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os_,
+                                              B, Hq, Hkv, Sq, Sk, D, window, sinks, mp, ms, scale, _ptr(ws), need,
+                                              _stream_ptr(q)), "rldx_window_attention_bf16")
+    return out
+
+
+def kv4_cache(num_pages: int, kv_heads: int, head_dim: int, *, page_tokens: int = 64, device="cuda") -> torch.Tensor:
+    """Pages for K/V rows in 4 bits (MXFP4: 17/32 byte per value), [num_pages, kv_heads, bytes of a page] uint8,
+    uninitialised.  page_tokens: a power of two, 32 or more; head_dim 64 or 128 (rldx_kv4_cache_t)."""
+    n = int(_lib.load().rldx_kv4_page_bytes(page_tokens, head_dim))
+    _require(n > 0, "kv4_cache: page_tokens must be a power of two from 32 on, head_dim 64 or 128")
+    return torch.empty((num_pages, kv_heads, n), dtype=torch.uint8, device=device)
+
+
+def _kv4(cache, page_table, starts, counts, B: int, heads: Optional[int], D: int):
+    """rldx_kv4_cache_t of checked tensors."""
+    _require(cache.dtype == torch.uint8 and cache.dim() == 3 and cache.stride(2) == 1,
+             "cache must be a kv4_cache(): uint8 [pages, kv_heads, bytes]")
+    _require(D in (64, 128), "head_dim must be 64 or 128")
+    tokens = cache.shape[2] // (34 * D) * 32
+    _require(tokens >= 32 and tokens & (tokens - 1) == 0 and cache.shape[2] == tokens // 32 * 34 * D,
+             f"cache pages of {cache.shape[2]} bytes are not those of head_dim {D}")
+    _require(heads is None or cache.shape[1] == heads, "cache and rows must have the same kv heads")
+    _require(page_table.dtype == torch.int32 and page_table.dim() == 2 and page_table.shape[0] == B and
+             (page_table.stride(1) == 1 or page_table.shape[1] <= 1), "page_table must be int32 [B, pages], rows contiguous")
+    _require(page_table.shape[1] * tokens <= 1 << 30, "page_table: at most 2^30 slots per sequence")
+    for t, n in ((starts, "starts"), (counts, "counts")):
+        _require(t is None or (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()), f"{n} must be int32 [B]")
+    st = [cache.stride(i) if cache.shape[i] > 1 else cache.shape[2] for i in range(2)]
+    _require(st[0] % 16 == 0 and st[1] % 16 == 0 and st[0] >= cache.shape[2] and st[1] >= cache.shape[2] and
+             (cache.data_ptr() % 16 == 0 or cache.numel() == 0), "cache pages must be 16-byte aligned and apart")
+    return _lib.Kv4Cache(_ptr(cache), cache.shape[0], cache.shape[1], D, tokens, *st, _ptr(page_table),
+                         page_table.shape[1], page_table.stride(0))
+
+
+def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+               counts: Optional[torch.Tensor] = None) -> None:
+    """Writes rows k, v [B, S, Hkv, D] bf16 to the slots starts[b] + i (i < counts[b], or all S) of the cache, in 4
+    bits.  page_table int32 [B, pages]: slot s of sequence b is in page page_table[b, s // page_tokens]; slots below 0
+    or of missing pages (past the table, ids outside the cache) are skipped.  No two rows of a call may have the same
+    slot.  Blocks of 32 with an infinity or a NaN read back as NaN (rldx_kv4_append_bf16)."""
+    _on_gpu(cache, k, v, page_table, starts, counts)
+    ks, vs = _rows4(k, "k"), _rows4(v, "v")
+    _require(k.shape == v.shape, "k and v must have one shape")
+    B, S, H, D = k.shape
+    c = _kv4(cache, page_table, starts, counts, B, H, D)
+    if k.numel() == 0:
+        return
+    lib = _lib.load()
+    _lib.check(lib.rldx_kv4_append_bf16(c, k.data_ptr(), ks, v.data_ptr(), vs, starts.data_ptr(), _ptr(counts), B, S,
+                                        _stream_ptr(k)), "rldx_kv4_append_bf16")
+
+
+def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, count: int, head_dim: int):
+    """(k, v) [B, count, Hkv, D] bf16: what the slots starts[b] .. + count - 1 stand for, exactly; NaN for slots below
+    0 or of missing pages (rldx_kv4_read_bf16)."""
+    _on_gpu(cache, page_table, starts)
+    _require(starts.dim() == 1 and count >= 0, "starts must be int32 [B], count at least 0")
+    B = starts.shape[0]
+    c = _kv4(cache, page_table, starts, None, B, None, head_dim)
+    k = torch.empty((B, count, cache.shape[1], head_dim), dtype=BF16, device=cache.device)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        return k, v
+    lib = _lib.load()
+    st = _rows4(k, "k")
+    _lib.check(lib.rldx_kv4_read_bf16(c, starts.data_ptr(), k.data_ptr(), st, v.data_ptr(), st, B, count, _stream_ptr(k)),
+               "rldx_kv4_read_bf16")
+    return k, v
+
+
+def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+                  counts: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                  scale: Optional[float] = None, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, Sq, Hq, D] bf16 over the 4-bit cache (see kv4_append, which has written the queries' own
+    K / V rows) -> [B, Sq, Hq, D].  Query i of sequence b stands at slot p = starts[b] + i and sees slot j iff j <= p
+    and (window None, or j > p - window, or j < sinks); queries i >= counts[b] get zeros.  A query that sees a slot of
+    a missing page gets NaN; pages that no query sees are not touched (rldx_kv4_attention_bf16)."""
+    _on_gpu(q, cache, page_table, starts, counts, out)
+    qs = _rows4(q, "q")
+    B, Sq, Hq, D = q.shape
+    c = _kv4(cache, page_table, starts, counts, B, None, D)
+    Hkv = cache.shape[1]
+    _require(Hkv > 0 and Hq % Hkv == 0, "q heads must be a multiple of kv heads")
+    window, sinks = NO_WINDOW if window is None else int(window), int(sinks)
+    _require(window >= 1 and sinks >= 0, "window must be at least 1, sinks at least 0")
+    scale = _softmax_scale(scale, D)
+    out = _out4(q, out)
+    os_ = _rows4(out, "out")
+    if out.numel() == 0:
+        return out
+    lib = _lib.load()
+    need = int(lib.rldx_kv4_attention_workspace_bytes(B, Hq, Hkv, Sq, D, c.page_tokens, c.table_pages, window, sinks))
+    _require(need >= 0, "kv4_attention: sizes out of range (Sq * Hq / Hkv up to 2^30)")
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _lib.check(lib.rldx_kv4_attention_bf16(q.data_ptr(), qs, c, starts.data_ptr(), _ptr(counts), out.data_ptr(), os_, B,
+                                           Hq, Sq, window, sinks, scale, _ptr(ws), need, _stream_ptr(q)),
+               "rldx_kv4_attention_bf16")
+    return out
+
+
 def vision_attention_workspace_bytes(total_tokens: int, num_seqs: int, num_heads: int, head_dim: int) -> int:
     n = int(_lib.load().rldx_vision_attention_workspace_bytes(total_tokens, num_seqs, num_heads, head_dim))
     _require(n >= 0, f"vision attention: unsupported head_dim {head_dim} (multiple of 8 in [8, 128])")

@@ -10,6 +10,8 @@ Importing this module registers, backed by the gfx950 kernels of librldx_amd.so:
   rldx_backbone::fused_epilogue_add2_rmsnorm   rldx_backbone::fused_epilogue_add3_rmsnorm
   mem::fused_epilogue_add2_rmsnorm
   rldx_amd::swiglu           (the eager `F.silu(x1) * x2` the chains inline)
+  rldx_amd::window_attention   rldx_amd::kv4_append   rldx_amd::kv4_read   rldx_amd::kv4_attention
+                             (a stream of tokens: sliding window with sinks, 4-bit K/V cache; not in the reference)
 
 Argument order and defaults follow the reference registrations
 (rldx/inference/action_model/{double,single}_stream/engine/ops/*.py,
@@ -339,6 +341,62 @@ def swiglu_op(x: torch.Tensor) -> torch.Tensor:
 @swiglu_op.register_fake
 def _(x):
     return x.new_empty((*x.shape[:-1], x.shape[-1] // 2))
+
+
+# ---------------------------------------------------------------------------
+# rldx_amd::  attention over a stream of tokens: sliding window, 4-bit K/V cache
+# ---------------------------------------------------------------------------
+
+
+@torch.library.custom_op("rldx_amd::window_attention", mutates_args=())
+def window_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0,
+                        key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Causal GQA attention of the last Sq of Sk tokens with a sliding window and the first `sinks` keys
+    (functional.window_attention)."""
+    return Fn.window_attention(q, k, v, window, sinks, key_mask, scale)
+
+
+@window_attention_op.register_fake
+def _(q, k, v, window, sinks=0, key_mask=None, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("rldx_amd::kv4_append", mutates_args=("cache",))
+def kv4_append_op(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
+                  starts: torch.Tensor, counts: Optional[torch.Tensor] = None) -> None:
+    """K/V rows into a paged cache in 4 bits (functional.kv4_append)."""
+    Fn.kv4_append(cache, k, v, page_table, starts, counts)
+
+
+@kv4_append_op.register_fake
+def _(cache, k, v, page_table, starts, counts=None):
+    return None
+
+
+@torch.library.custom_op("rldx_amd::kv4_read", mutates_args=())
+def kv4_read_op(cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, count: int,
+                head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values that slots of the cache stand for (functional.kv4_read)."""
+    return Fn.kv4_read(cache, page_table, starts, count, head_dim)
+
+
+@kv4_read_op.register_fake
+def _(cache, page_table, starts, count, head_dim):
+    shape = (starts.shape[0], count, cache.shape[1], head_dim)
+    return cache.new_empty(shape, dtype=torch.bfloat16), cache.new_empty(shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("rldx_amd::kv4_attention", mutates_args=())
+def kv4_attention_op(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor,
+                     counts: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """Attention over the 4-bit cache, single tokens or chunks (functional.kv4_attention)."""
+    return Fn.kv4_attention(q, cache, page_table, starts, counts, window, sinks, scale)
+
+
+@kv4_attention_op.register_fake
+def _(q, cache, page_table, starts, counts=None, window=None, sinks=0, scale=None):
+    return q.new_empty(q.shape)
 
 
 # ---------------------------------------------------------------------------
