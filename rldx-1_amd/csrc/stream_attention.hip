@@ -26,6 +26,8 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -144,9 +146,38 @@ __device__ __forceinline__ bf16x8 dequant8(uint32_t c, float s) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// (The pairs are opaque to the compiler in these three, or it works them out ahead for every tile, and keeps registers
+// for them, though only a few tiles come here.)
 __device__ __forceinline__ bool nonfinite2(uint32_t w) {  // either half of a bf16 pair
-  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+  asm volatile("" : "+v"(w));
+  const bool hi = (w & 0x7f800000u) == 0x7f800000u, lo = (w & 0x7f80u) == 0x7f80u;
+  return hi || lo;
 }
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {  // with zeros in the place of what is not
+  asm volatile("" : "+v"(w));
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+  return w;
+}
+// 1.0 where a half of the pair is of kind 0 .. 3 (+inf, -inf, NaN, NaN with a sign), else 0.
+__device__ __forceinline__ uint32_t marks2(uint32_t w, int kind) {
+  asm volatile("" : "+v"(w));
+  const uint32_t base = (kind & 1 ? 0xff80u : 0x7f80u) + (kind >> 1), more = kind >> 1 ? 0x7eu : 0u;
+  return ((w & 0xffffu) - base <= more ? 0x3f80u : 0u) | ((w >> 16) - base <= more ? 0x3f800000u : 0u);
+}
+__device__ __forceinline__ float mark_value(int kind) {
+  return kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
+}
+
+// The keys 0 .. 31 of a tile that a query sees, a bit each: k0 <= p, and k0 > p - window or k0 < sinks.
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+__device__ __forceinline__ uint32_t visible_bits(int k0, int p, int window, int sinks) {
+  return below(p + 1 - k0) & (~below(p + 1 - window - k0) | below(sinks - k0));
+}
+
+// Factor of a state whose reference moves from m to n >= m.  Never 0: an infinity in O has to stay one, and what is
+// scaled by 2^-126 is lost beside the new terms just as well.  (No reference yet: O and the sum are 0.)
+__device__ __forceinline__ float rescale(float m, float n) { return __builtin_amdgcn_exp2f(fmaxf(m - n, -126.f)); }
 
 // NT: 16-row blocks of a workgroup.
 template <int D, int NT, bool kCache>
@@ -272,19 +303,16 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
 
   floatx4 oacc[NT][W];
   float m_ref[NT], l[NT];
-  bool poison[NT];  // a visible V block of this lane's dimensions is NaN, or the query stands past the limit
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int j = 0; j < W; ++j) oacc[nt][j] = floatx4{0, 0, 0, 0};
     m_ref[nt] = -__builtin_inff();
     l[nt] = 0.f;
-    poison[nt] = pos[nt] >= a.limit;
   }
 
   // every query of the block sees something (the columns past the last row repeat it)
   const bool all_rows = sp.p0 == sp.start + row0 / a.group && sp.p1 == sp.start + (min(row0 + RB, rows) - 1) / a.group;
-  auto visible = [&](int key, int p) { return key <= p && (key > p - a.window || key < a.sinks); };
 
   auto compute = [&](Raw<D, kCache>& raw, int it, int page) {
     const int k0 = tile_at(it) * kTile;
@@ -327,35 +355,43 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
       }
     }
     // ---- visibility ----
-    bool odd_v = false;  // (wave-uniform) the tile's V holds something that is not finite: handled key by key
-    if (!full) {
+    bool odd_v = false;  // (wave-uniform) the tile's V holds something that is not finite
+    uint32_t vis[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) vis[nt] = ~0u;
+    if (!full) {
+      uint32_t mbits = ~0u;  // bits 4 g .. + 3 and 16 + 4 g .. + 3: the others are not looked at
+      if constexpr (!kCache) {
+        if (a.mask) {
+          mbits = 0;
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mbits |= (raw.m[kt][r] != 0.f ? 1u : 0u) << (kt * 16 + g * 4 + r);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        vis[nt] = (visible_bits(k0, pos[nt], a.window, a.sinks) & mbits) >> (4 * g);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            bool ok = visible(k0 + kt * 16 + g * 4 + r, pos[nt]);
-            if constexpr (!kCache) ok = ok && (!a.mask || raw.m[kt][r] != 0.f);
             const float sc = kCache && page < 0 ? __builtin_nanf("") : s[nt][kt][r];
-            s[nt][kt][r] = ok ? sc : -__builtin_inff();
+            s[nt][kt][r] = vis[nt] & (1u << (16 * kt + r)) ? sc : -__builtin_inff();
           }
-      if constexpr (kCache) {
-        bool dirty = false;
+      }
+      bool dirty = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t e = (raw.vs[i >> 2] >> (8 * (i & 3))) & 255u;
-          dirty |= e >= 253;
-        }
-        odd_v = __any(dirty);
-      } else {
-        bool dirty = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (kCache) {
+          dirty |= ((raw.vs[i >> 2] >> (8 * (i & 3))) & 255u) >= 253u;  // an element may be one
+        } else {
 #pragma unroll
           for (int j = 0; j < W / 2; ++j) dirty |= nonfinite2(raw.v[i][j]);
-        odd_v = __any(dirty);
+        }
       }
+      odd_v = __any(dirty);
     }
     // ---- softmax ----
     bf16x8 pf[NT];
@@ -366,7 +402,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
       mt *= a.scale_log2;
       if (__any(mt > m_ref[nt] + kMoveRef)) {
         const float nr = fmaxf(m_ref[nt], quad_max(mt));
-        const float al = m_ref[nt] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_ref[nt] - nr);
+        const float al = rescale(m_ref[nt], nr);
         m_ref[nt] = nr;
         l[nt] *= al;
 #pragma unroll
@@ -411,21 +447,41 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
             vr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1));
           }
         }
-        if (odd_v && e >= 253) {
-#pragma unroll
-          for (int j = 0; j < W / 2; ++j) vr[i][j] = 0;
-        }
       } else {
 #pragma unroll
-        for (int j = 0; j < W / 2; ++j) {
-          uint32_t w = raw.v[i][j];
-          if (odd_v) {
-            if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
-            if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
-          }
-          vr[i][j] = w;
-        }
+        for (int j = 0; j < W / 2; ++j) vr[i][j] = raw.v[i][j];
       }
+    }
+    if (odd_v) {
+      // Infinities and NaN of V go to the queries that see them, by products of what marks them with the visible
+      // keys, and leave zeros behind: a key that a query does not see weighs 0, and 0 times them would be NaN.
+#pragma unroll 1
+      for (int kind = 0; kind < 4; ++kind)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          u32x4 vf;
+#pragma unroll
+          for (int tp = 0; tp < 4; ++tp)
+            vf[tp] = marks2(perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u), kind);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            u32x4 seen;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int c = 16 * (x >> 1) + 2 * (x & 1);
+              seen[x] = (vis[nt] & (1u << c) ? 0x3f80u : 0u) | (vis[nt] & (2u << c) ? 0x3f800000u : 0u);
+            }
+            const floatx4 z = {0, 0, 0, 0};
+            const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf),
+                                                                        __builtin_bit_cast(bf16x8, seen), z, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) oacc[nt][j][r] += hit[r] > 0.f ? mark_value(kind) : 0.f;
+          }
+        }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < W / 2; ++j) vr[i][j] = finite2(vr[i][j]);
     }
     // ---- O^T += V^T P^T ----
 #pragma unroll
@@ -437,41 +493,6 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         oacc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf), pf[nt], oacc[nt][j], 0, 0, 0);
-    }
-    if (odd_v) {
-      // what the products above left out, for the queries that see it: this lane's dimensions are
-      // 4 W g .. 4 W g + 4 W - 1, O^T element (j, r) the one at W r + j among them
-      if constexpr (kCache) {
-        const uint8_t* const t = a.cache + page * a.page_stride + hk * a.head_stride +
-                                 ((k0 & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
-        for (int key = 0; page >= 0 && key < kTile; ++key) {
-          const uint32_t e = t[33 * D + (4 * W * g / 32 * 4 + kv4::v_group(key)) * 8 + kv4::v_unit(key)];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) poison[nt] = poison[nt] || (e >= 253 && visible(k0 + key, pos[nt]));
-        }
-      } else {
-        const uint16_t* const vb = a.v + b * a.v_sb + hk * a.v_sh + 4 * W * g;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; ++r4)
-            for (int gg = 0; gg < 4; ++gg) {
-              const int key = k0 + kt * 16 + gg * 4 + r4;
-              if (key >= a.limit || (a.mask && a.mask[b * a.mask_sb + key] == 0.f)) continue;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const float pr = __shfl(s[nt][kt][r4], n16 + 16 * gg);
-                if (!visible(key, pos[nt])) continue;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                  for (int j = 0; j < W; ++j) {
-                    const uint16_t x = vb[key * a.v_ss + W * r + j];
-                    if ((x & 0x7f80) == 0x7f80) oacc[nt][j][r] += pr * bf16_bits_to_f32(x);
-                  }
-              }
-            }
-      }
     }
   };
 
@@ -503,7 +524,8 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
 #pragma unroll
       for (int j = 0; j < W; j += 4) {
         floatx4 x = {oacc[nt][j][r], oacc[nt][j + 1][r], oacc[nt][j + 2][r], oacc[nt][j + 3][r]};
-        if (poison[nt]) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+        // (a query past the limit sees slots that nobody can read)
+        if (kCache && pos[nt] >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
         *reinterpret_cast<floatx4*>(&sm_o[wave][n16][4 * W * g + W * r + j]) = x;
       }
     if (g == 0) {
@@ -518,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
       for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) {
-        w[i] = sm_ml[i][mr][0] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sm_ml[i][mr][0] - m);
+        w[i] = rescale(sm_ml[i][mr][0], m);
         lt = __builtin_fmaf(sm_ml[i][mr][1], w[i], lt);
       }
       float acc[W];
@@ -556,6 +578,450 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many query rows: 128 (token, head) rows of a KV head's group per workgroup, 32 a wave, and tiles of 32
+// keys that the workgroup brings into LDS once: bf16 rows straight from memory (buffer_load ... lds, three slots
+// ahead of the matrix work), codes of the cache through registers, as the bf16 values they stand for.
+//   S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16_bf16: a lane owns a query column, so maxima, sums and
+//   rescaling stay in the lane and its partner (lane ^ 32), and P^T goes from accumulator to operand in place.
+//   Both operands lie in LDS as rows, 16-byte pieces of row r exchanged by an XOR: K's by r mod the pieces of a row
+//   (a lane reads one piece of its own key: 8 lanes cover 8 bank groups), V's by 2 (r mod 4) (ds_read_b64_tr_b16
+//   gathers 4 keys of 16 dimensions, 32 bytes of each of 4 rows, into the V^T operand).
+// Rows in (token, head) order keep the workgroup's windows together: 128 rows of 4 heads a group span 32 tokens, so
+// a window of 1024 takes 34 tiles of which every wave needs 33.
+// ---------------------------------------------------------------------------
+template <int N>
+__device__ __forceinline__ void vm_wait_barrier() {  // all but this wave's last N loads have arrived, everywhere
+  static_assert(N == 0 || N == 2 || N == 4, "vmcnt immediate");
+  if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ float pair_max(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
+}
+
+// 16 bytes from base + offset of every lane to LDS, lane after lane (base: uniform).
+__device__ __forceinline__ void load_lds16(const void* base, uint8_t* lds, int offset) {
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
+}
+
+// The V^T operands of two 32-dimension blocks: rows 8 x .. 8 x + 7 of LDS through the transposing read, x < 4.  The
+// reads and their wait are one block: beside builtins of these reads the compiler waits for every load into LDS that is
+// still in flight.
+template <int ROWB>
+__device__ __forceinline__ void read_v(u32x2 (&v0)[2][2], u32x2 (&v1)[2][2], uint32_t at0, uint32_t at1) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %9\n\t"
+      "ds_read_b64_tr_b16 %5, %9 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %6, %9 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %7, %9 offset:%12\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v0[0][0]), "=&v"(v0[0][1]), "=&v"(v0[1][0]), "=&v"(v0[1][1]), "=&v"(v1[0][0]), "=&v"(v1[0][1]),
+        "=&v"(v1[1][0]), "=&v"(v1[1][1])
+      : "v"(at0), "v"(at1), "n"(8 * ROWB), "n"(16 * ROWB), "n"(24 * ROWB)
+      : "memory");
+}
+
+template <int D, bool kCache, bool kMask>
+__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
+  constexpr int RB = 128;
+  constexpr int KCH = D / 16;      // MFMA steps over head_dim
+  constexpr int DBLK = D / 32;     // 32-dimension blocks of O^T
+  constexpr int PCS = D / 8;       // 16-byte pieces of a row
+  constexpr int ROWB = 2 * D;      // bytes of a row
+  constexpr int CH = 32 * ROWB / 1024;   // 1 KB chunks of a tile's K or V
+  constexpr int CPW = CH / kWaves;       // of them a wave loads (D = 64: one)
+  constexpr int NS = kCache ? 2 : 3;     // ring slots
+  constexpr int OP = D + 8;              // pitch of O rows staged in LDS
+  constexpr int RING = NS * 64 * ROWB, STAGE = kWaves * 32 * OP * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t ring[RING > STAGE ? RING : STAGE];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+  const int l32 = lane & 31, g = lane >> 5;
+
+  // work item: (batch, kv head, row tile, split), neighbours on one XCD (workgroup i runs on XCD i % 8)
+  int id;
+  {
+    const int total = static_cast<int>(gridDim.x), i = static_cast<int>(blockIdx.x);
+    const int per = total / 8, rem = total % 8, xcd = i % 8, k = i / 8;
+    id = xcd < rem ? xcd * (per + 1) + k : rem * (per + 1) + (xcd - rem) * per + k;
+  }
+  const int split = id % a.splits;
+  id /= a.splits;
+  const int rt = id % a.row_tiles;
+  id /= a.row_tiles;
+  const int hk = id % a.hkv, b = id / a.hkv;
+
+  const int rows = a.sq * a.group;
+  const int row0 = rt * RB, rw0 = row0 + 32 * wave;
+  const Span sp = span_of<kCache>(a, b, row0, min(RB, rows - row0));
+  const int use = splits_of(a.splits, sp.n);
+  if (split >= use) return;
+  const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
+  const int n = static_cast<int>(static_cast<int64_t>(sp.n) * (split + 1) / use) - t0;
+  auto tile_at = [&](int it) {
+    const int t = t0 + it;
+    return t < sp.ns ? t : sp.w0 + (t - sp.ns);
+  };
+
+  // this lane's query, and the first and last slot of the wave's queries
+  const int row = min(rw0 + l32, rows - 1);
+  const int qi = row / a.group, qh = hk * a.group + row - qi * a.group;
+  const int pos = qi < sp.count ? max(sp.start + qi, -1) : -1;
+  const int pw0 = sp.start + rw0 / a.group, pw1 = sp.start + (min(rw0 + 32, rows) - 1) / a.group;
+  // (every query of the wave sees something)
+  const bool all_rows = rw0 < rows && pw0 >= 0 && pw0 >= sp.p0 && pw1 <= sp.p1;
+  bf16x8 qf[KCH];
+  {
+    const uint16_t* const src = a.q + b * a.q_sb + qi * a.q_ss + qh * a.q_sh + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KCH; ++ks) qf[ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + 16 * ks));
+  }
+
+  // ---- tiles into LDS ----
+  const uint16_t* const kb = kCache ? nullptr : a.k + b * a.k_sb + hk * a.k_sh;
+  const uint16_t* const vb = kCache ? nullptr : a.v + b * a.v_sb + hk * a.v_sh;
+  auto swz_k = [](int r) { return r & (PCS - 1); };
+  auto swz_v = [](int r) { return 2 * (r & 3); };
+  // this lane's rows and pieces of the wave's chunks
+  int drow[CPW], dk[CPW], dv[CPW];
+#pragma unroll
+  for (int c = 0; c < CPW; ++c) {
+    drow[c] = (wave + kWaves * c) * (1024 / ROWB) + lane / PCS;
+    dk[c] = drow[c] * static_cast<int>(a.k_ss * 2) + ((lane % PCS) ^ swz_k(drow[c])) * 16;
+    dv[c] = drow[c] * static_cast<int>(a.v_ss * 2) + ((lane % PCS) ^ swz_v(drow[c])) * 16;
+  }
+  auto dma = [&](int tile, int slot) {
+    const int k0 = tile * kTile;
+    // (rows of less than 2^25 bytes: the step from tile to tile has 31 bits)
+    const uint8_t* const kt = reinterpret_cast<const uint8_t*>(kb) +
+                              static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.k_ss * (2 * kTile));
+    const uint8_t* const vt = reinterpret_cast<const uint8_t*>(vb) +
+                              static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.v_ss * (2 * kTile));
+    uint8_t* const to = ring + slot * 64 * ROWB + wave * 1024;
+    int ok[CPW], ov[CPW];
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) ok[c] = dk[c], ov[c] = dv[c];
+    if (k0 + kTile > a.limit) {  // rows past the last key repeat it
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) {
+        const int past = max(drow[c] - (a.limit - 1 - k0), 0);
+        ok[c] -= past * static_cast<int>(a.k_ss * 2);
+        ov[c] -= past * static_cast<int>(a.v_ss * 2);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) load_lds16(kt, to + kWaves * c * 1024, ok[c]);
+#pragma unroll
+    for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + kWaves * c * 1024, ov[c]);
+  };
+  // page ids of 64 tiles, one a lane
+  int ids = -1, ids_base = 0;
+  auto load_ids = [&](int it0) {
+    ids_base = it0;
+    ids = -1;
+    if constexpr (kCache) {
+      const int it = it0 + lane;
+      if (it < n) ids = a.table[b * a.table_sb + ((tile_at(it) * kTile) >> a.page_shift)];
+    }
+  };
+  auto page_of = [&](int it) {  // called with it ascending
+    if (it - ids_base >= 64) load_ids(it);
+    const int page = __builtin_amdgcn_readlane(ids, it - ids_base);
+    return page < a.num_pages ? max(page, -1) : -1;
+  };
+  auto tile_ptr = [&](int page, int it) {
+    return a.cache + page * a.page_stride + hk * a.head_stride +
+           (((tile_at(it) * kTile) & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
+  };
+  // threads 0 .. 127 take K, D / 4 dimensions of a row each, the others V, a quarter of the lane blocks' units
+  const int ct = static_cast<int>(threadIdx.x) & 127;
+  u32x4 codes;
+  uint32_t scales;
+  auto fetch = [&](int page, int it) {
+    codes = u32x4{0, 0, 0, 0};
+    scales = 0;
+    if (page < 0) return;
+    const uint8_t* const t = tile_ptr(page, it);
+    const uint8_t* const src = t + (wave < 2 ? 0 : 16 * D) + ct * (D / 8);
+    if constexpr (D == 128) {
+      codes = *reinterpret_cast<const u32x4*>(src);
+    } else {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(src);
+      codes = u32x4{x[0], x[1], 0, 0};
+    }
+    if (wave < 2) {
+      scales = t[32 * D + (ct >> 2) * (D / 32) + (D == 128 ? ct & 3 : (ct & 3) >> 1)];
+    } else {  // the scales of 4 slots
+      const int lb = ct >> 1;
+      scales = *reinterpret_cast<const uint32_t*>(t + 33 * D + ((lb & 15) * (D / 16) / 32 * 4 + (lb >> 4)) * 8 + (ct & 1) * 4);
+    }
+  };
+  auto store = [&](int slot) {
+    uint8_t* const ks = ring + slot * 64 * ROWB;
+    if (wave < 2) {
+      const int r = ct >> 2;
+      const float sc = __builtin_bit_cast(float, scales << 23);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint32_t c = codes[j];
+        const int piece = (ct & 3) * (D / 32) + j;
+        *reinterpret_cast<bf16x8*>(ks + r * ROWB + (piece ^ swz_k(r)) * 16) = dequant8(c, sc);
+      }
+    } else {
+      const int lb = ct >> 1;
+      const int r0 = 16 * (ct & 1) + 4 * (lb >> 4), col = lb & 15;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + j;
+        const float sc = __builtin_bit_cast(float, ((scales >> (8 * j)) & 255u) << 23);
+        uint8_t* const dst = ks + 32 * ROWB + r * ROWB;
+        if constexpr (D == 128) {
+          const uint32_t c = codes[j];
+          *reinterpret_cast<bf16x8*>(dst + (col ^ swz_v(r)) * 16) = dequant8(c, sc);
+        } else {
+          uint32_t c = codes[j >> 1];
+          c = j & 1 ? c >> 16 : c;
+          const u32x2 x = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0)),
+                           __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1))};
+          *reinterpret_cast<u32x2*>(dst + ((col >> 1) ^ swz_v(r)) * 16 + (col & 1) * 8) = x;
+        }
+      }
+    }
+  };
+
+  floatx16 oacc[DBLK];
+#pragma unroll
+  for (int db = 0; db < DBLK; ++db) oacc[db] = floatx16{};
+  float m_ref = -__builtin_inff(), l = 0.f;
+
+  // the mask of a tile's keys, a bit each (lane l < 32 loads key l's, a step ahead)
+  float mload = 1.f;
+  auto fetch_mask = [&](int tile) {
+    if constexpr (kMask) mload = a.mask[b * a.mask_sb + min(tile * kTile + l32, a.limit - 1)];
+  };
+
+  // this lane's part of a V^T operand's addresses: 8 bytes of row 4 g + (lane / 4) % 4 of every 8 rows
+  const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)ring));
+  const uint32_t v_row = (4 * g + ((lane >> 2) & 3)) * ROWB + (lane & 1) * 8;
+  const int v_piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), v_swz = 2 * ((lane >> 2) & 3);
+
+  auto compute = [&](int k0, int slot, int page, uint32_t mbits) {
+    if (k0 > pw1 || (k0 + kTile - 1 <= pw0 - a.window && k0 >= a.sinks) || rw0 >= rows) return;
+    if (kMask && mbits == 0) return;
+    const uint8_t* const ks = ring + slot * 64 * ROWB;
+    // ---- S^T ----
+    floatx16 s = floatx16{};
+    {
+      u32x4 kop[KCH];
+#pragma unroll
+      for (int c = 0; c < KCH; ++c) kop[c] = *reinterpret_cast<const u32x4*>(ks + l32 * ROWB + ((2 * c + g) ^ swz_k(l32)) * 16);
+#pragma unroll
+      for (int c = 0; c < KCH; ++c)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], s, 0, 0, 0);
+    }
+    // ---- V^T: keys 16 s2 + 8 h + 4 g .. + 3 of dimension 32 db + l32 ----
+    u32x2 vop[DBLK][2][2];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int db = 0; db < DBLK; db += 2) {
+      const uint32_t vaddr = ring_at + slot * 64 * ROWB + 32 * ROWB + v_row + ((4 * db + v_piece) ^ v_swz) * 16;
+      const uint32_t vaddr1 = ring_at + slot * 64 * ROWB + 32 * ROWB + v_row + ((4 * db + 4 + v_piece) ^ v_swz) * 16;
+      read_v<ROWB>(vop[db], vop[db + 1], vaddr, vaddr1);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- visibility ----
+    const bool full = all_rows && page >= 0 && mbits == 0xffffffffu && k0 + kTile - 1 <= pw0 &&
+                      (k0 > pw1 - a.window || k0 + kTile <= a.sinks);
+    bool odd_v = false;
+    uint32_t vis = ~0u;
+    if (!full) {
+      vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float sc = kCache && page < 0 ? __builtin_nanf("") : s[e];
+        s[e] = vis & (1u << (8 * (e >> 2) + (e & 3))) ? sc : -__builtin_inff();
+      }
+      bool dirty = false;
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            dirty |= nonfinite2(vop[db][s2][h][0]);
+            dirty |= nonfinite2(vop[db][s2][h][1]);
+          }
+      odd_v = __any(dirty);
+    }
+    // ---- softmax ----
+    float mt = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[e]);
+    mt *= a.scale_log2;
+    if (__any(mt > m_ref + kMoveRef)) {
+      const float nr = fmaxf(m_ref, pair_max(mt));
+      const float al = rescale(m_ref, nr);
+      m_ref = nr;
+      l *= al;
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db) oacc[db] *= al;
+    }
+    const float nm = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+    float ps = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, nm));
+      ps += s[e];
+    }
+    l += ps;
+    if (odd_v) {  // (as in rows_attn_kernel)
+#pragma unroll 1
+      for (int kind = 0; kind < 4; ++kind)
+#pragma unroll
+        for (int db = 0; db < DBLK; ++db) {
+          floatx16 hit = floatx16{};
+#pragma unroll
+          for (int s2 = 0; s2 < 2; ++s2) {
+            u32x4 vf, seen;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              vf[x] = marks2(vop[db][s2][x >> 1][x & 1], kind);
+              const int c = 16 * s2 + 8 * (x >> 1) + 2 * (x & 1);
+              seen[x] = (vis & (1u << c) ? 0x3f80u : 0u) | (vis & (2u << c) ? 0x3f800000u : 0u);
+            }
+            hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, seen),
+                                                          hit, 0, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) oacc[db][e] += hit[e] > 0.f ? mark_value(kind) : 0.f;
+        }
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) vop[db][s2][h][x] = finite2(vop[db][s2][h][x]);
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const u32x4 pk = {pack_bf16x2(s[8 * s2], s[8 * s2 + 1]), pack_bf16x2(s[8 * s2 + 2], s[8 * s2 + 3]),
+                        pack_bf16x2(s[8 * s2 + 4], s[8 * s2 + 5]), pack_bf16x2(s[8 * s2 + 6], s[8 * s2 + 7])};
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db) {
+        const u32x4 vf = {vop[db][s2][0][0], vop[db][s2][0][1], vop[db][s2][1][0], vop[db][s2][1][1]};
+        oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pk),
+                                                           oacc[db], 0, 0, 0);
+      }
+    }
+  };
+
+  if (n > 0) {
+    if constexpr (kCache) {
+      load_ids(0);
+      int pg0 = page_of(0), pg1 = -1;
+      fetch(pg0, 0);
+      store(0);
+      if (n > 1) {
+        pg1 = page_of(1);
+        fetch(pg1, 1);
+      }
+      for (int it = 0; it < n; ++it) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        int pg2 = -1;
+        if (it + 1 < n) store((it + 1) & 1);
+        if (it + 2 < n) {
+          pg2 = page_of(it + 2);
+          fetch(pg2, it + 2);
+        }
+        compute(tile_at(it) * kTile, it & 1, pg0, 0xffffffffu);
+        pg0 = pg1;
+        pg1 = pg2;
+      }
+    } else {
+      // tiles of the steps it, it + 1, it + 2 (past the end: the last one again)
+      const int t_last = tile_at(n - 1);
+      auto next = [&](int t) { return t == t_last ? t : t + 1 == sp.ns ? sp.w0 : t + 1; };
+      int ta = tile_at(0), tb = next(ta), tc = next(tb);
+      dma(ta, 0);
+      fetch_mask(ta);
+      dma(tb, 1);
+      int slot = 0;
+      for (int it = 0; it < n; ++it) {
+        vm_wait_barrier<2 * CPW>();  // tile it is in LDS, the slot of tile it - 1 is free
+        uint32_t mbits = 0xffffffffu;
+        if constexpr (kMask) mbits = static_cast<uint32_t>(__ballot(mload != 0.f));
+        fetch_mask(tb);
+        dma(tc, slot == 0 ? 2 : slot - 1);
+        compute(ta * kTile, slot, 0, mbits);
+        slot = slot == 2 ? 0 : slot + 1;
+        ta = tb;
+        tb = tc;
+        tc = next(tc);
+      }
+    }
+  }
+  vm_wait_barrier<0>();  // every wave has read its last tile, no load into LDS is in flight
+
+  const float lt = pair_sum(l);
+  if (a.splits > 1) {
+    if (rw0 + l32 < rows) {
+      const int64_t item = (((static_cast<int64_t>(b) * a.hkv + hk) * a.row_tiles + rt) * a.splits + split) * RB + 32 * wave + l32;
+      const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * RB;
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          floatx4 x = {oacc[db][4 * q4], oacc[db][4 * q4 + 1], oacc[db][4 * q4 + 2], oacc[db][4 * q4 + 3]};
+          if (kCache && pos >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+          *reinterpret_cast<floatx4*>(a.part + item * D + 32 * db + 8 * q4 + 4 * g) = x;
+        }
+      if (g == 0) {
+        a.part[items * D + item * 2] = m_ref;
+        a.part[items * D + item * 2 + 1] = lt;
+      }
+    }
+    return;
+  }
+  float inv = lt > 0.f ? 1.f / lt : lt == 0.f ? 1.f : lt;
+  if (kCache && pos >= a.limit) inv = __builtin_nanf("");  // (sees slots that nobody can read)
+  uint16_t* const st = reinterpret_cast<uint16_t*>(ring) + wave * (32 * OP);
+#pragma unroll
+  for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<u32x2*>(st + l32 * OP + 32 * db + 8 * q4 + 4 * g) =
+          u32x2{pack_bf16x2(oacc[db][4 * q4] * inv, oacc[db][4 * q4 + 1] * inv),
+                pack_bf16x2(oacc[db][4 * q4 + 2] * inv, oacc[db][4 * q4 + 3] * inv)};
+  // whole rows in 16-byte pieces (a wave reads what it wrote itself)
+#pragma unroll
+  for (int x = 0; x < 32 * PCS / 64; ++x) {
+    const int r = x * (64 / PCS) + lane / PCS, c = lane % PCS * 8;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(st + r * OP + c);
+    const int orow = rw0 + r;
+    if (orow >= rows) continue;
+    const int i = orow / a.group, h = hk * a.group + orow - i * a.group;
+    *reinterpret_cast<u32x4*>(a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + c) = w;
+  }
+}
+
 // O of a query row from the partial states of its splits: wave w adds up splits w, w + 4, ...
 template <int D, bool kCache>
 __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb) {
@@ -582,7 +1048,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb
   float top = m;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-  const float w = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+  const float w = rescale(m, top);
   l *= w;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
@@ -627,9 +1093,9 @@ bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How a call is cut up; depends on sizes alone.
 struct Plan {
-  int nt, row_tiles, splits;
+  int rb, row_tiles, splits;  // rows of a workgroup: 16, 32, 64 (rows_attn_kernel) or 128 (tile_attn_kernel)
   int64_t items;  // row blocks times splits
-  int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * 16 * nt * (head_dim + 2) * 4 : 0; }
+  int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * rb * (head_dim + 2) * 4 : 0; }
 };
 
 // limit: readable keys.  false: sizes that the kernels do not take.
@@ -640,15 +1106,15 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     return false;
   const int64_t group = q_heads / kv_heads, rows = seq_q * group;
   if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
-  p.nt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int64_t rb = 16 * p.nt;
+  p.rb = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const int64_t rb = p.rb;
   p.row_tiles = static_cast<int>(rows == 0 ? 1 : (rows + rb - 1) / rb);
   const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * p.row_tiles);
   // tiles of the longest row block
   const int64_t span = std::min(limit, std::min(window, limit) + rb / std::max<int64_t>(1, group) + 1);
   const int64_t tiles = std::min((limit + kTile - 1) / kTile,
                                  (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
-  const int64_t want = std::max<int64_t>(1, (p.nt == 4 ? 256 : 512) / blocks);
+  const int64_t want = std::max<int64_t>(1, (p.rb >= 64 ? 256 : 512) / blocks);
   p.splits = static_cast<int>(std::min<int64_t>({64, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
   p.items = blocks * p.splits;
   return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
@@ -681,16 +1147,23 @@ void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* 
 template <int D, bool kCache>
 hipError_t launch_rows(const StreamArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.items)), block(64 * kWaves);
-  if (p.nt == 1)
+  if (p.rb == 128) {
+    if constexpr (kCache)
+      hipLaunchKernelGGL((tile_attn_kernel<D, true, false>), grid, block, 0, stream, a);
+    else if (a.mask)
+      hipLaunchKernelGGL((tile_attn_kernel<D, false, true>), grid, block, 0, stream, a);
+    else
+      hipLaunchKernelGGL((tile_attn_kernel<D, false, false>), grid, block, 0, stream, a);
+  } else if (p.rb == 16)
     hipLaunchKernelGGL((rows_attn_kernel<D, 1, kCache>), grid, block, 0, stream, a);
-  else if (p.nt == 2)
+  else if (p.rb == 32)
     hipLaunchKernelGGL((rows_attn_kernel<D, 2, kCache>), grid, block, 0, stream, a);
   else
     hipLaunchKernelGGL((rows_attn_kernel<D, 4, kCache>), grid, block, 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>(a.batch * a.hq * a.sq)), block, 0, stream, a,
-                     16 * p.nt);
+                     p.rb);
   return hipGetLastError();
 }
 
@@ -723,6 +1196,9 @@ extern "C" hipError_t rldx_window_attention_bf16(const void* q, const int64_t* q
   if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks) ||
       !common_ok(q, q_strides, o, o_strides, scale) || !strides_ok(k_strides) || !strides_ok(v_strides) || !a16(k) ||
       !a16(v) || reinterpret_cast<uintptr_t>(key_mask) % 4)
+    return hipErrorInvalidValue;
+  // (a tile's rows are addressed with 32-bit byte offsets)
+  if (k_strides[1] < 0 || v_strides[1] < 0 || k_strides[1] > (1 << 24) || v_strides[1] > (1 << 24))
     return hipErrorInvalidValue;
   if (batch == 0 || q_heads == 0 || seq_q == 0) return hipSuccess;
   if (!q || !k || !v || !o) return hipErrorInvalidValue;
