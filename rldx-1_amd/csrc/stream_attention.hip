@@ -35,7 +35,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = kv4::kTile;
 constexpr int kWaves = 4;
 constexpr int kMaxSlots = 1 << 30;
-constexpr float kMoveRef = 3.f;  // log2 units: the softmax reference moves when a score exceeds it by 2^3
+constexpr float kMoveRef = 5.f;  // log2 units: the softmax reference moves when a score exceeds it by 2^5
 
 struct StreamArgs {
   const uint16_t* q;
@@ -645,10 +645,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   constexpr int ROWB = 2 * D;      // bytes of a row
   constexpr int CH = 32 * ROWB / 1024;   // 1 KB chunks of a tile's K or V
   constexpr int CPW = CH / kWaves;       // of them a wave loads (D = 64: one)
-  constexpr int NS = kCache ? 2 : 3;     // ring slots
+  constexpr int TILEB = 2 * 32 * ROWB;   // K and V of a tile in LDS; a ring slot holds two tiles, a step's
   constexpr int OP = D + 8;              // pitch of O rows staged in LDS
-  constexpr int RING = NS * 64 * ROWB, STAGE = kWaves * 32 * OP * 2;
-  __shared__ __attribute__((aligned(16))) uint8_t ring[RING > STAGE ? RING : STAGE];
+  constexpr int RING = 2 * 2 * TILEB, STAGE = kWaves * 32 * OP * 2;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[RING > STAGE ? RING : STAGE];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l32 = lane & 31, g = lane >> 5;
@@ -705,14 +705,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
     dk[c] = drow[c] * static_cast<int>(a.k_ss * 2) + ((lane % PCS) ^ swz_k(drow[c])) * 16;
     dv[c] = drow[c] * static_cast<int>(a.v_ss * 2) + ((lane % PCS) ^ swz_v(drow[c])) * 16;
   }
-  auto dma = [&](int tile, int slot) {
+  auto dma = [&](int tile, int off) {  // off: of the tile's place in LDS
     const int k0 = tile * kTile;
     // (rows of less than 2^25 bytes: the step from tile to tile has 31 bits)
     const uint8_t* const kt = reinterpret_cast<const uint8_t*>(kb) +
                               static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.k_ss * (2 * kTile));
     const uint8_t* const vt = reinterpret_cast<const uint8_t*>(vb) +
                               static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.v_ss * (2 * kTile));
-    uint8_t* const to = ring + slot * 64 * ROWB + wave * 1024;
+    uint8_t* const to = ring + off + wave * 1024;
     int ok[CPW], ov[CPW];
 #pragma unroll
     for (int c = 0; c < CPW; ++c) ok[c] = dk[c], ov[c] = dv[c];
@@ -750,9 +750,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   };
   // threads 0 .. 127 take K, D / 4 dimensions of a row each, the others V, a quarter of the lane blocks' units
   const int ct = static_cast<int>(threadIdx.x) & 127;
-  u32x4 codes;
-  uint32_t scales;
-  auto fetch = [&](int page, int it) {
+  auto fetch = [&](int page, int it, u32x4& codes, uint32_t& scales) {
     codes = u32x4{0, 0, 0, 0};
     scales = 0;
     if (page < 0) return;
@@ -771,8 +769,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
       scales = *reinterpret_cast<const uint32_t*>(t + 33 * D + ((lb & 15) * (D / 16) / 32 * 4 + (lb >> 4)) * 8 + (ct & 1) * 4);
     }
   };
-  auto store = [&](int slot) {
-    uint8_t* const ks = ring + slot * 64 * ROWB;
+  auto store = [&](int off, u32x4 codes, uint32_t scales) {
+    uint8_t* const ks = ring + off;
     if (wave < 2) {
       const int r = ct >> 2;
       const float sc = __builtin_bit_cast(float, scales << 23);
@@ -809,48 +807,148 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   for (int db = 0; db < DBLK; ++db) oacc[db] = floatx16{};
   float m_ref = -__builtin_inff(), l = 0.f;
 
-  // the mask of a tile's keys, a bit each (lane l < 32 loads key l's, a step ahead)
+  // the mask of a step's keys, a bit each (lanes 0 .. 31 load the first tile's, the others the second's, a step ahead)
   float mload = 1.f;
-  auto fetch_mask = [&](int tile) {
-    if constexpr (kMask) mload = a.mask[b * a.mask_sb + min(tile * kTile + l32, a.limit - 1)];
+  auto fetch_mask = [&](int ta, int tb) {
+    if constexpr (kMask) mload = a.mask[b * a.mask_sb + min((g ? tb : ta) * kTile + l32, a.limit - 1)];
   };
 
-  // this lane's part of a V^T operand's addresses: 8 bytes of row 4 g + (lane / 4) % 4 of every 8 rows
+  // LDS addresses of this lane's part of the operands: piece g of row l32 of K; 8 bytes of row 4 g + (lane / 4) % 4 of
+  // every 8 rows of V (piece 2 (lane / 16 % 2) + lane / 2 % 2)
   const uint32_t ring_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)ring));
-  const uint32_t v_row = (4 * g + ((lane >> 2) & 3)) * ROWB + (lane & 1) * 8;
-  const int v_piece = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1), v_swz = 2 * ((lane >> 2) & 3);
+  const uint32_t k_at = ring_at + l32 * ROWB + (g ^ swz_k(l32)) * 16;
+  const uint32_t v_at = ring_at + 32 * ROWB + (4 * g + ((lane >> 2) & 3)) * ROWB + (lane & 1) * 8 +
+                        ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ swz_v(lane >> 2)) * 16;
 
-  auto compute = [&](int k0, int slot, int page, uint32_t mbits) {
-    if (k0 > pw1 || (k0 + kTile - 1 <= pw0 - a.window && k0 >= a.sinks) || rw0 >= rows) return;
+  auto skipped = [&](int k0) { return k0 > pw1 || (k0 + kTile - 1 <= pw0 - a.window && k0 >= a.sinks) || rw0 >= rows; };
+  // every query of the wave sees all 32 keys
+  auto whole = [&](int k0) {
+    const bool low = k0 > pw1 - a.window, sink = k0 + kTile <= a.sinks, high = k0 + kTile - 1 <= pw0;
+    return all_rows & high & (low | sink);
+  };
+  auto load_k = [&](u32x4 (&kop)[KCH], int off) {
+    // (piece 2 c + g is the swizzled piece g with 2 c exchanged too: one address and an XOR for each)
+    const uint32_t at = k_at + off;
+#pragma unroll
+    for (int c = 0; c < KCH; ++c)
+      kop[c] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(at ^ (32 * c));
+  };
+  auto load_v = [&](u32x2 (&vop)[DBLK][2][2], int off) {
+    const uint32_t at = v_at + off;
+#pragma unroll
+    for (int db = 0; db < DBLK; db += 2) read_v<ROWB>(vop[db], vop[db + 1], at ^ (64 * db), at ^ (64 * db + 64));
+  };
+  auto top_of = [&](const floatx16& s) {
+    float mt = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[e]);
+    return mt * a.scale_log2;
+  };
+  auto move_ref = [&](float mt) {
+    const float nr = fmaxf(m_ref, pair_max(mt));
+    const float al = rescale(m_ref, nr);
+    m_ref = nr;
+    l *= al;
+#pragma unroll
+    for (int db = 0; db < DBLK; ++db) oacc[db] *= al;
+    return al;
+  };
+  auto exp_all = [&](floatx16& s) {
+    const float nm = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+    float ps = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, nm));
+      ps += s[e];
+    }
+    l += ps;
+  };
+  auto pack = [&](const floatx16& s, u32x4 (&pk)[2]) {
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+      pk[s2] = u32x4{pack_bf16x2(s[8 * s2], s[8 * s2 + 1]), pack_bf16x2(s[8 * s2 + 2], s[8 * s2 + 3]),
+                     pack_bf16x2(s[8 * s2 + 4], s[8 * s2 + 5]), pack_bf16x2(s[8 * s2 + 6], s[8 * s2 + 7])};
+  };
+  auto pv = [&](const u32x2 (&vop)[DBLK][2][2], const u32x4 (&pk)[2]) {
+#pragma unroll
+    for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+      for (int db = 0; db < DBLK; ++db) {
+        const u32x4 vf = {vop[db][s2][0][0], vop[db][s2][0][1], vop[db][s2][1][0], vop[db][s2][1][1]};
+        oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pk[s2]),
+                                                           oacc[db], 0, 0, 0);
+      }
+  };
+  // one matrix instruction, then its share of the 56 vector instructions (16 of them exponentials) of a tile's softmax
+  auto interleave = [&]() {
+#pragma unroll
+    for (int i = 0; i < KCH; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 40 / KCH, 0);
+      __builtin_amdgcn_sched_group_barrier(0x400, 16 / KCH, 0);
+    }
+  };
+
+  // Two tiles that the wave's queries see whole: the softmax of each between matrix instructions of the other.
+  auto compute2 = [&](int off) {
+    u32x4 kop[KCH], pa[2], pb[2];
+    u32x2 vop[DBLK][2][2];
+    floatx16 sa = floatx16{}, sb = floatx16{};
+    load_k(kop, off);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < KCH; ++c)
+      sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], sa, 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(kop, off + TILEB);
+    const float ma = top_of(sa);
+    if (__any(ma > m_ref + kMoveRef)) move_ref(ma);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = 0; c < KCH; ++c)
+      sb = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], sb, 0, 0, 0);
+    exp_all(sa);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(vop, off);
+    __builtin_amdgcn_sched_barrier(0);
+    const float mb = top_of(sb);
+    if (__any(mb > m_ref + kMoveRef)) sa *= move_ref(mb);
+    __builtin_amdgcn_sched_barrier(0);
+    pack(sa, pa);
+    pv(vop, pa);
+    exp_all(sb);
+    pack(sb, pb);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(vop, off + TILEB);
+    __builtin_amdgcn_sched_barrier(0);
+    pv(vop, pb);
+  };
+
+  bool odd_v = false;  // (wave-uniform) some tile's V held infinities or NaN that not every query of the wave sees
+
+  // Any tile.
+  auto compute = [&](int k0, int off, int page, uint32_t mbits) {
+    if (skipped(k0)) return;
     if (kMask && mbits == 0) return;
-    const uint8_t* const ks = ring + slot * 64 * ROWB;
-    // ---- S^T ----
     floatx16 s = floatx16{};
+    u32x2 vop[DBLK][2][2];
     {
       u32x4 kop[KCH];
-#pragma unroll
-      for (int c = 0; c < KCH; ++c) kop[c] = *reinterpret_cast<const u32x4*>(ks + l32 * ROWB + ((2 * c + g) ^ swz_k(l32)) * 16);
+      load_k(kop, off);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int c = 0; c < KCH; ++c)
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], s, 0, 0, 0);
     }
-    // ---- V^T: keys 16 s2 + 8 h + 4 g .. + 3 of dimension 32 db + l32 ----
-    u32x2 vop[DBLK][2][2];
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int db = 0; db < DBLK; db += 2) {
-      const uint32_t vaddr = ring_at + slot * 64 * ROWB + 32 * ROWB + v_row + ((4 * db + v_piece) ^ v_swz) * 16;
-      const uint32_t vaddr1 = ring_at + slot * 64 * ROWB + 32 * ROWB + v_row + ((4 * db + 4 + v_piece) ^ v_swz) * 16;
-      read_v<ROWB>(vop[db], vop[db + 1], vaddr, vaddr1);
-    }
+    load_v(vop, off);
     __builtin_amdgcn_sched_barrier(0);
     // ---- visibility ----
-    const bool full = all_rows && page >= 0 && mbits == 0xffffffffu && k0 + kTile - 1 <= pw0 &&
-                      (k0 > pw1 - a.window || k0 + kTile <= a.sinks);
-    bool odd_v = false;
-    uint32_t vis = ~0u;
+    const bool full = whole(k0) && page >= 0 && mbits == 0xffffffffu;
     if (!full) {
-      vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
+      const uint32_t vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float sc = kCache && page < 0 ? __builtin_nanf("") : s[e];
@@ -866,119 +964,148 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
             dirty |= nonfinite2(vop[db][s2][h][0]);
             dirty |= nonfinite2(vop[db][s2][h][1]);
           }
-      odd_v = __any(dirty);
-    }
-    // ---- softmax ----
-    float mt = s[0];
+      if (__any(dirty)) {
+        // A key that a query does not see weighs 0, and 0 times an infinity or a NaN is a NaN: they go to the queries
+        // that see them behind the loop, and count as zeros here.
+        odd_v = true;
 #pragma unroll
-    for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[e]);
-    mt *= a.scale_log2;
-    if (__any(mt > m_ref + kMoveRef)) {
-      const float nr = fmaxf(m_ref, pair_max(mt));
-      const float al = rescale(m_ref, nr);
-      m_ref = nr;
-      l *= al;
+        for (int db = 0; db < DBLK; ++db)
 #pragma unroll
-      for (int db = 0; db < DBLK; ++db) oacc[db] *= al;
-    }
-    const float nm = m_ref == -__builtin_inff() ? 0.f : -m_ref;
-    float ps = 0.f;
+          for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, nm));
-      ps += s[e];
-    }
-    l += ps;
-    if (odd_v) {  // (as in rows_attn_kernel)
-#pragma unroll 1
-      for (int kind = 0; kind < 4; ++kind)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int db = 0; db < DBLK; ++db) {
-          floatx16 hit = floatx16{};
-#pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) {
-            u32x4 vf, seen;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              vf[x] = marks2(vop[db][s2][x >> 1][x & 1], kind);
-              const int c = 16 * s2 + 8 * (x >> 1) + 2 * (x & 1);
-              seen[x] = (vis & (1u << c) ? 0x3f80u : 0u) | (vis & (2u << c) ? 0x3f800000u : 0u);
-            }
-            hit = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, seen),
-                                                          hit, 0, 0, 0);
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) oacc[db][e] += hit[e] > 0.f ? mark_value(kind) : 0.f;
-        }
-#pragma unroll
-      for (int db = 0; db < DBLK; ++db)
-#pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) vop[db][s2][h][x] = finite2(vop[db][s2][h][x]);
-    }
-    // ---- O^T += V^T P^T ----
-#pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2) {
-      const u32x4 pk = {pack_bf16x2(s[8 * s2], s[8 * s2 + 1]), pack_bf16x2(s[8 * s2 + 2], s[8 * s2 + 3]),
-                        pack_bf16x2(s[8 * s2 + 4], s[8 * s2 + 5]), pack_bf16x2(s[8 * s2 + 6], s[8 * s2 + 7])};
-#pragma unroll
-      for (int db = 0; db < DBLK; ++db) {
-        const u32x4 vf = {vop[db][s2][0][0], vop[db][s2][0][1], vop[db][s2][1][0], vop[db][s2][1][1]};
-        oacc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pk),
-                                                           oacc[db], 0, 0, 0);
+              for (int x = 0; x < 2; ++x) vop[db][s2][h][x] = finite2(vop[db][s2][h][x]);
       }
     }
+    const float mt = top_of(s);
+    if (__any(mt > m_ref + kMoveRef)) move_ref(mt);
+    u32x4 pk[2];
+    exp_all(s);
+    pack(s, pk);
+    pv(vop, pk);
   };
 
   if (n > 0) {
+    // Steps of two tiles in the two slots of the ring.  begin(st): step st's tiles are in LDS, the next ones on their way.
+    const int steps = (n + 1) / 2;
+    struct Step {
+      int k0, k1;      // first keys of the two tiles (an odd number of tiles: the last step has no second one)
+      int p0, p1;      // their pages, -1: missing (kCache)
+      uint64_t mask;   // of their 64 keys (kMask)
+      bool pair;       // a step for compute2
+    };
+    auto step = [&](int st, int k0, int k1, int p0, int p1, uint64_t mask) {
+      bool two = 2 * st + 1 < n;
+      two &= whole(k0);
+      two &= whole(k1);
+      two &= p0 >= 0;
+      two &= p1 >= 0;
+      two &= mask == ~uint64_t{0};
+      return Step{k0, k1, p0, p1, mask, two};
+    };
+    auto run = [&](auto begin) {
+      int st = 0;
+      Step x = begin(0);
+      // (two loops, so that the state does not change registers at every step)
+      while (st < steps) {
+        while (st < steps && !x.pair) {
+          const int off = (st & 1) * 2 * TILEB;
+          compute(x.k0, off, x.p0, static_cast<uint32_t>(x.mask));
+          if (2 * st + 1 < n) compute(x.k1, off + TILEB, x.p1, static_cast<uint32_t>(x.mask >> 32));
+          if (++st < steps) x = begin(st);
+        }
+        while (st < steps && x.pair) {
+          compute2((st & 1) * 2 * TILEB);
+          if (++st < steps) x = begin(st);
+        }
+      }
+    };
     if constexpr (kCache) {
       load_ids(0);
-      int pg0 = page_of(0), pg1 = -1;
-      fetch(pg0, 0);
-      store(0);
-      if (n > 1) {
-        pg1 = page_of(1);
-        fetch(pg1, 1);
-      }
-      for (int it = 0; it < n; ++it) {
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        int pg2 = -1;
-        if (it + 1 < n) store((it + 1) & 1);
-        if (it + 2 < n) {
-          pg2 = page_of(it + 2);
-          fetch(pg2, it + 2);
+      u32x4 codes[2];
+      uint32_t scales[2];
+      int page[2], page_next[2] = {-1, -1};
+      auto fetch2 = [&](int st, int (&pg)[2]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          pg[x] = 2 * st + x < n ? page_of(2 * st + x) : -1;
+          fetch(pg[x], 2 * st + x, codes[x], scales[x]);
         }
-        compute(tile_at(it) * kTile, it & 1, pg0, 0xffffffffu);
-        pg0 = pg1;
-        pg1 = pg2;
-      }
+      };
+      auto store2 = [&](int slot) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) store((2 * slot + x) * TILEB, codes[x], scales[x]);
+      };
+      fetch2(0, page);
+      store2(0);
+      if (steps > 1) fetch2(1, page_next);
+      run([&](int st) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int p0 = page[0], p1 = page[1];
+        if (st + 1 < steps) store2((st + 1) & 1);
+        page[0] = page_next[0], page[1] = page_next[1];
+        if (st + 2 < steps) fetch2(st + 2, page_next);
+        return step(st, tile_at(2 * st) * kTile, tile_at(2 * st + 1) * kTile, p0, p1, ~uint64_t{0});
+      });
     } else {
-      // tiles of the steps it, it + 1, it + 2 (past the end: the last one again)
+      // tiles of this step and the next one (past the end: the last one again)
       const int t_last = tile_at(n - 1);
       auto next = [&](int t) { return t == t_last ? t : t + 1 == sp.ns ? sp.w0 : t + 1; };
-      int ta = tile_at(0), tb = next(ta), tc = next(tb);
+      int ta = tile_at(0), tb = next(ta);
+      fetch_mask(ta, tb);
       dma(ta, 0);
-      fetch_mask(ta);
-      dma(tb, 1);
-      int slot = 0;
-      for (int it = 0; it < n; ++it) {
-        vm_wait_barrier<2 * CPW>();  // tile it is in LDS, the slot of tile it - 1 is free
-        uint32_t mbits = 0xffffffffu;
-        if constexpr (kMask) mbits = static_cast<uint32_t>(__ballot(mload != 0.f));
-        fetch_mask(tb);
-        dma(tc, slot == 0 ? 2 : slot - 1);
-        compute(ta * kTile, slot, 0, mbits);
-        slot = slot == 2 ? 0 : slot + 1;
-        ta = tb;
-        tb = tc;
-        tc = next(tc);
-      }
+      dma(tb, TILEB);
+      run([&](int st) {
+        vm_wait_barrier<0>();  // the step's tiles are in LDS, the other slot is free
+        uint64_t mask = ~uint64_t{0};
+        if constexpr (kMask) mask = __ballot(mload != 0.f);
+        const Step x = step(st, ta * kTile, tb * kTile, 0, 0, mask);
+        ta = next(tb), tb = next(ta);
+        if (st + 1 < steps) {
+          const int to = ((st + 1) & 1) * 2 * TILEB;
+          fetch_mask(ta, tb);
+          dma(ta, to);
+          dma(tb, to + TILEB);
+        }
+        return x;
+      });
     }
   }
   vm_wait_barrier<0>();  // every wave has read its last tile, no load into LDS is in flight
+
+  if (__builtin_expect(odd_v, 0)) {
+    for (int it = 0; it < n; ++it) {
+      const int k0 = tile_at(it) * kTile;
+      if (skipped(k0)) continue;
+      uint32_t mbits = ~0u;
+      if constexpr (kMask) mbits = static_cast<uint32_t>(__ballot(a.mask[b * a.mask_sb + min(k0 + l32, a.limit - 1)] != 0.f));
+      if (mbits == 0 || (whole(k0) && mbits == ~0u)) continue;  // (whole tiles: the products have them)
+      uint32_t vis = visible_bits(k0, pos, a.window, a.sinks) & mbits;
+      if constexpr (kCache) {
+        const int page = __builtin_amdgcn_readfirstlane(a.table[b * a.table_sb + (k0 >> a.page_shift)]);
+        if (page < 0 || page >= a.num_pages) continue;
+        const uint8_t* const sc = tile_ptr(page, it) + 33 * D;
+        for (; vis; vis &= vis - 1) {
+          const int key = __builtin_ctz(vis);
+#pragma unroll
+          for (int db = 0; db < DBLK; ++db)
+            if (sc[(db * 4 + kv4::v_group(key)) * 8 + kv4::v_unit(key)] >= 253) oacc[db] += __builtin_nanf("");
+        }
+      } else {
+        for (; vis; vis &= vis - 1) {
+          const uint16_t* const src = vb + static_cast<int64_t>(k0 + __builtin_ctz(vis)) * a.v_ss + 4 * g;
+#pragma unroll
+          for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const uint16_t w = src[32 * db + 8 * (x >> 2) + (x & 3)];
+              if ((w & 0x7f80) == 0x7f80) oacc[db][x] += bf16_bits_to_f32(w);
+            }
+        }
+      }
+    }
+  }
 
   const float lt = pair_sum(l);
   if (a.splits > 1) {
