@@ -27,6 +27,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -34,6 +35,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = kv4::kTile;
 constexpr int kWaves = 4;
+constexpr int kRowsBlock = 16;  // rows of a rows_attn_kernel workgroup
 constexpr int kMaxSlots = 1 << 30;
 constexpr float kMoveRef = 5.f;  // log2 units: the softmax reference moves when a score exceeds it by 2^5
 
@@ -119,8 +121,6 @@ __device__ __forceinline__ float quad_sum(float x) {
   return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
 }
 
-__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
-
 // What a lane loads of a tile of 32 keys.
 template <int D, bool kCache>
 struct Raw;
@@ -146,13 +146,17 @@ __device__ __forceinline__ bf16x8 dequant8(uint32_t c, float s) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// (The pairs are opaque to the compiler in these three, or it works them out ahead for every tile, and keeps registers
-// for them, though only a few tiles come here.)
-__device__ __forceinline__ bool nonfinite2(uint32_t w) {  // either half of a bf16 pair
-  asm volatile("" : "+v"(w));
-  const bool hi = (w & 0x7f800000u) == 0x7f800000u, lo = (w & 0x7f80u) == 0x7f80u;
-  return hi || lo;
-}
+// (The pairs are opaque to the compiler in these, or it works them out ahead for every tile, and keeps registers for
+// them, though only a few tiles come here.)
+// The largest magnitude of bf16 values, whose bits order as they do: an infinity or a NaN is 0x7f80 or more.
+struct Largest {
+  u16x2 m = {0, 0};
+  __device__ __forceinline__ void look(uint32_t w) {
+    asm volatile("" : "+v"(w));
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+  }
+  __device__ __forceinline__ bool nonfinite() const { return (m[0] >= 0x7f80) | (m[1] >= 0x7f80); }
+};
 __device__ __forceinline__ uint32_t finite2(uint32_t w) {  // with zeros in the place of what is not
   asm volatile("" : "+v"(w));
   if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
@@ -178,32 +182,29 @@ __device__ __forceinline__ uint32_t visible_bits(int k0, int p, int window, int 
 // Factor of a state whose reference moves from m to n >= m.  Never 0: an infinity in O has to stay one, and what is
 // scaled by 2^-126 is lost beside the new terms just as well.  (No reference yet: O and the sum are 0.)
 __device__ __forceinline__ float rescale(float m, float n) { return __builtin_amdgcn_exp2f(fmaxf(m - n, -126.f)); }
+// 1 / sum of a softmax: a query that has seen nothing has O = 0; a NaN stays.
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : l == 0.f ? 1.f : l; }
 
-// NT: 16-row blocks of a workgroup.
-template <int D, int NT, bool kCache>
-__global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel(StreamArgs a) {
-  constexpr int RB = 16 * NT;
-  constexpr int KS = D / 32;   // MFMA steps over head_dim
-  constexpr int W = D / 16;    // dimensions of a lane's V columns, blocks of O^T
-  constexpr int OP = D + 4;    // pitch of O in LDS (floats)
+template <int D, bool kCache>
+__global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a) {
+  constexpr int KS = D / 32;          // MFMA steps over head_dim
+  constexpr int W = D / 16;           // dimensions of a lane's V columns, blocks of O^T
+  constexpr int OP = D + 4;           // pitch of O in LDS (floats)
   constexpr int PF = kCache ? 2 : 1;  // tiles a wave has in flight
-  __shared__ __attribute__((aligned(16))) float sm_o[kWaves][16][OP];
-  __shared__ float sm_ml[kWaves][16][2];
+  __shared__ __attribute__((aligned(16))) float sm_o[kWaves][kRowsBlock][OP];
+  __shared__ float sm_ml[kWaves][kRowsBlock][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int n16 = lane & 15, g = lane >> 4;
 
-  // work item: (batch, kv head, split, row tile)
+  // work item: (batch, kv head, split)
   int id = static_cast<int>(blockIdx.x);
-  const int rt = id % a.row_tiles;
-  id /= a.row_tiles;
   const int split = id % a.splits;
   id /= a.splits;
   const int hk = id % a.hkv, b = id / a.hkv;
 
-  const int rows = a.sq * a.group;
-  const int row0 = rt * RB;
-  const Span sp = span_of<kCache>(a, b, row0, min(RB, rows - row0));
+  const int rows = a.sq * a.group;  // <= kRowsBlock
+  const Span sp = span_of<kCache>(a, b, 0, rows);
   const int use = splits_of(a.splits, sp.n);
   if (split >= use) return;
   const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
@@ -214,18 +215,18 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
     return t < sp.ns ? t : sp.w0 + (t - sp.ns);
   };
 
-  // this lane's queries: column n16 of each 16-row block
-  int pos[NT];      // slot, -1: sees nothing
-  bf16x8 qf[NT][KS];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = min(row0 + 16 * nt + n16, rows - 1);
-    const int i = r / a.group, h = hk * a.group + r - i * a.group;
-    pos[nt] = i < sp.count ? max(sp.start + i, -1) : -1;
-    const uint16_t* const src = a.q + b * a.q_sb + i * a.q_ss + h * a.q_sh + (kCache ? D / 4 : 8) * g;
+  // this lane's query: column n16 (the columns past the last row repeat it, and are not stored)
+  const int row = min(n16, rows - 1);
+  const int qi = row / a.group, qh = hk * a.group + row - qi * a.group;
+  const int pos = qi < sp.count ? max(sp.start + qi, -1) : -1;  // slot, -1: sees nothing
+  // every query sees something
+  const bool all_rows = sp.p0 == sp.start && sp.p1 == sp.start + a.sq - 1;
+  bf16x8 qf[KS];
+  {
+    const uint16_t* const src = a.q + b * a.q_sb + qi * a.q_ss + qh * a.q_sh + (kCache ? D / 4 : 8) * g;
 #pragma unroll
     for (int s = 0; s < KS; ++s)
-      qf[nt][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + (kCache ? 8 : 32) * s));
+      qf[s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(src + (kCache ? 8 : 32) * s));
   }
 
   // page ids of the wave's next 64 tiles, one a lane
@@ -257,14 +258,14 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
                                ((k0 & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const int row = kt * 16 + n16;
+        const int r = kt * 16 + n16;
         if constexpr (D == 128) {
-          raw.k[kt] = *reinterpret_cast<const u32x4*>(t + row * 64 + g * 16);
-          raw.ks[kt] = t[32 * D + row * 4 + g];
+          raw.k[kt] = *reinterpret_cast<const u32x4*>(t + r * 64 + g * 16);
+          raw.ks[kt] = t[32 * D + r * 4 + g];
         } else {
-          const u32x2 c = *reinterpret_cast<const u32x2*>(t + row * 32 + g * 8);
+          const u32x2 c = *reinterpret_cast<const u32x2*>(t + r * 32 + g * 8);
           raw.k[kt] = u32x4{c[0], c[1], 0, 0};
-          raw.ks[kt] = t[32 * D + row * 2 + (g >> 1)];
+          raw.ks[kt] = t[32 * D + r * 2 + (g >> 1)];
         }
       }
       raw.v[0] = *reinterpret_cast<const u32x4*>(t + 16 * D + lane * (D / 4));
@@ -301,22 +302,14 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
     }
   };
 
-  floatx4 oacc[NT][W];
-  float m_ref[NT], l[NT];
+  floatx4 oacc[W];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int j = 0; j < W; ++j) oacc[nt][j] = floatx4{0, 0, 0, 0};
-    m_ref[nt] = -__builtin_inff();
-    l[nt] = 0.f;
-  }
-
-  // every query of the block sees something (the columns past the last row repeat it)
-  const bool all_rows = sp.p0 == sp.start + row0 / a.group && sp.p1 == sp.start + (min(row0 + RB, rows) - 1) / a.group;
+  for (int j = 0; j < W; ++j) oacc[j] = floatx4{0, 0, 0, 0};
+  float m_ref = -__builtin_inff(), l = 0.f;
 
   auto compute = [&](Raw<D, kCache>& raw, int it, int page) {
     const int k0 = tile_at(it) * kTile;
-    // every query of the block sees all 32 keys: no masks, and no key whose V may not be touched
+    // every query sees all 32 keys: no masks, and no key whose V may not be touched
     bool full = page >= 0 && all_rows && k0 + kTile - 1 <= sp.p0 && (k0 > sp.p1 - a.window || k0 + kTile <= a.sinks);
     if constexpr (!kCache) {
       if (a.mask) {
@@ -333,11 +326,10 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
       }
     }
     // ---- S^T ----
-    floatx4 s[NT][2];
+    floatx4 s[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][kt] = floatx4{0, 0, 0, 0};
+      s[kt] = floatx4{0, 0, 0, 0};
       float ks = 0.f;
       if constexpr (kCache) ks = __builtin_bit_cast(float, raw.ks[kt] << 23);
 #pragma unroll
@@ -349,16 +341,12 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
         } else {
           kf = __builtin_bit_cast(bf16x8, raw.k[kt][st]);
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          s[nt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][st], s[nt][kt], 0, 0, 0);
+        s[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[st], s[kt], 0, 0, 0);
       }
     }
     // ---- visibility ----
     bool odd_v = false;  // (wave-uniform) the tile's V holds something that is not finite
-    uint32_t vis[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) vis[nt] = ~0u;
+    uint32_t vis = ~0u;
     if (!full) {
       uint32_t mbits = ~0u;  // bits 4 g .. + 3 and 16 + 4 g .. + 3: the others are not looked at
       if constexpr (!kCache) {
@@ -370,17 +358,15 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
             for (int r = 0; r < 4; ++r) mbits |= (raw.m[kt][r] != 0.f ? 1u : 0u) << (kt * 16 + g * 4 + r);
         }
       }
+      vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        vis[nt] = (visible_bits(k0, pos[nt], a.window, a.sinks) & mbits) >> (4 * g);
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float sc = kCache && page < 0 ? __builtin_nanf("") : s[nt][kt][r];
-            s[nt][kt][r] = vis[nt] & (1u << (16 * kt + r)) ? sc : -__builtin_inff();
-          }
-      }
+        for (int r = 0; r < 4; ++r) {
+          const float sc = kCache && page < 0 ? __builtin_nanf("") : s[kt][r];
+          s[kt][r] = vis & (1u << (16 * kt + r)) ? sc : -__builtin_inff();
+        }
+      Largest big;
       bool dirty = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -388,42 +374,39 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
           dirty |= ((raw.vs[i >> 2] >> (8 * (i & 3))) & 255u) >= 253u;  // an element may be one
         } else {
 #pragma unroll
-          for (int j = 0; j < W / 2; ++j) dirty |= nonfinite2(raw.v[i][j]);
+          for (int j = 0; j < W / 2; ++j) {
+            const uint32_t w = raw.v[i][j];
+            big.look(w);
+          }
         }
       }
-      odd_v = __any(dirty);
+      odd_v = __any(dirty || big.nonfinite());
     }
     // ---- softmax ----
-    bf16x8 pf[NT];
+    float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+    mt *= a.scale_log2;
+    if (__any(mt > m_ref + kMoveRef)) {
+      const float nr = fmaxf(m_ref, quad_max(mt));
+      const float al = rescale(m_ref, nr);
+      m_ref = nr;
+      l *= al;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float mt = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
-                       fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
-      mt *= a.scale_log2;
-      if (__any(mt > m_ref[nt] + kMoveRef)) {
-        const float nr = fmaxf(m_ref[nt], quad_max(mt));
-        const float al = rescale(m_ref[nt], nr);
-        m_ref[nt] = nr;
-        l[nt] *= al;
-#pragma unroll
-        for (int j = 0; j < W; ++j) oacc[nt][j] *= al;
-      }
-      const float nm = m_ref[nt] == -__builtin_inff() ? 0.f : -m_ref[nt];
-      float ps = 0.f;
-      u32x4 pk;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[nt][kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[nt][kt][r], a.scale_log2, nm));
-          ps += s[nt][kt][r];
-        }
-        pk[2 * kt] = pack_bf16x2(s[nt][kt][0], s[nt][kt][1]);
-        pk[2 * kt + 1] = pack_bf16x2(s[nt][kt][2], s[nt][kt][3]);
-      }
-      l[nt] += ps;
-      pf[nt] = __builtin_bit_cast(bf16x8, pk);
+      for (int j = 0; j < W; ++j) oacc[j] *= al;
     }
+    const float nm = m_ref == -__builtin_inff() ? 0.f : -m_ref;
+    u32x4 pk;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[kt][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][r], a.scale_log2, nm));
+        l += s[kt][r];
+      }
+      pk[2 * kt] = pack_bf16x2(s[kt][0], s[kt][1]);
+      pk[2 * kt + 1] = pack_bf16x2(s[kt][2], s[kt][3]);
+    }
+    const bf16x8 pf = __builtin_bit_cast(bf16x8, pk);
     // ---- V rows of the lane's 8 keys, W dimensions each, in bf16 pairs ----
     uint32_t vr[8][W / 2];
 #pragma unroll
@@ -433,10 +416,9 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
         const float sc = __builtin_bit_cast(float, e << 23);
         if constexpr (D == 128) {
           const uint32_t c = raw.v[i >> 2][i & 3];
-          vr[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0));
-          vr[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1));
-          vr[i][2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2));
-          vr[i][3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3));
+          const u32x4 x = __builtin_bit_cast(u32x4, dequant8(c, sc));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vr[i][j] = x[j];
         } else {
           const uint32_t c = raw.v[0][i >> 1];
           if (i & 1) {
@@ -452,31 +434,35 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
         for (int j = 0; j < W / 2; ++j) vr[i][j] = raw.v[i][j];
       }
     }
+    // V^T operand of the block of dimensions W m + j, m < 16
+    auto turn = [&](int j) {
+      u32x4 vf;
+#pragma unroll
+      for (int tp = 0; tp < 4; ++tp)
+        vf[tp] = __builtin_amdgcn_perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+      return vf;
+    };
     if (odd_v) {
       // Infinities and NaN of V go to the queries that see them, by products of what marks them with the visible
       // keys, and leave zeros behind: a key that a query does not see weighs 0, and 0 times them would be NaN.
+      u32x4 seen;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int c = 16 * (x >> 1) + 2 * (x & 1);
+        seen[x] = (vis & (1u << c) ? 0x3f80u : 0u) | (vis & (2u << c) ? 0x3f800000u : 0u);
+      }
 #pragma unroll 1
       for (int kind = 0; kind < 4; ++kind)
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-          u32x4 vf;
+          u32x4 vf = turn(j);
 #pragma unroll
-          for (int tp = 0; tp < 4; ++tp)
-            vf[tp] = marks2(perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u), kind);
+          for (int tp = 0; tp < 4; ++tp) vf[tp] = marks2(vf[tp], kind);
+          const floatx4 zero = {0, 0, 0, 0};
+          const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf),
+                                                                      __builtin_bit_cast(bf16x8, seen), zero, 0, 0, 0);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            u32x4 seen;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int c = 16 * (x >> 1) + 2 * (x & 1);
-              seen[x] = (vis[nt] & (1u << c) ? 0x3f80u : 0u) | (vis[nt] & (2u << c) ? 0x3f800000u : 0u);
-            }
-            const floatx4 z = {0, 0, 0, 0};
-            const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf),
-                                                                        __builtin_bit_cast(bf16x8, seen), z, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) oacc[nt][j][r] += hit[r] > 0.f ? mark_value(kind) : 0.f;
-          }
+          for (int r = 0; r < 4; ++r) oacc[j][r] += hit[r] > 0.f ? mark_value(kind) : 0.f;
         }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -485,15 +471,8 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
     }
     // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      u32x4 vf;
-#pragma unroll
-      for (int tp = 0; tp < 4; ++tp)
-        vf[tp] = perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        oacc[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf), pf[nt], oacc[nt][j], 0, 0, 0);
-    }
+    for (int j = 0; j < W; ++j)
+      oacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, turn(j)), pf, oacc[j], 0, 0, 0);
   };
 
   Raw<D, kCache> raw[PF];
@@ -512,68 +491,62 @@ __global__ __launch_bounds__(64 * kWaves, NT == 4 ? 1 : 2) void rows_attn_kernel
     }
   }
 
-  // ---- merge the 4 waves, one 16-row block after the other ----
+  // ---- merge the 4 waves ----
+  const float lsum = quad_sum(l);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      floatx4 x = {oacc[j][r], oacc[j + 1][r], oacc[j + 2][r], oacc[j + 3][r]};
+      // (a query past the limit sees slots that nobody can read)
+      if (kCache && pos >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+      *reinterpret_cast<floatx4*>(&sm_o[wave][n16][4 * W * g + W * r + j]) = x;
+    }
+  if (g == 0) {
+    sm_ml[wave][n16][0] = m_ref;
+    sm_ml[wave][n16][1] = lsum;
+  }
+  __syncthreads();
   const int tid = static_cast<int>(threadIdx.x);
   const int mr = tid >> 4, md = (tid & 15) * W;  // the row and the first of W dimensions that this thread finishes
+  if (mr >= rows) return;
+  float m = -__builtin_inff(), lt = 0.f, w[kWaves];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float lsum = quad_sum(l[nt]);
-    if (nt) __syncthreads();
+  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+  for (int i = 0; i < kWaves; ++i) {
+    w[i] = rescale(sm_ml[i][mr][0], m);
+    lt = __builtin_fmaf(sm_ml[i][mr][1], w[i], lt);
+  }
+  float acc[W];
 #pragma unroll
-      for (int j = 0; j < W; j += 4) {
-        floatx4 x = {oacc[nt][j][r], oacc[nt][j + 1][r], oacc[nt][j + 2][r], oacc[nt][j + 3][r]};
-        // (a query past the limit sees slots that nobody can read)
-        if (kCache && pos[nt] >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-        *reinterpret_cast<floatx4*>(&sm_o[wave][n16][4 * W * g + W * r + j]) = x;
-      }
-    if (g == 0) {
-      sm_ml[wave][n16][0] = m_ref[nt];
-      sm_ml[wave][n16][1] = lsum;
-    }
-    __syncthreads();
-    const int row = row0 + 16 * nt + mr;
-    if (row < rows) {
-      float m = -__builtin_inff(), lt = 0.f, w[kWaves];
+  for (int j = 0; j < W; j += 4) {
+    floatx4 x = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
+    for (int i = 0; i < kWaves; ++i) x += *reinterpret_cast<const floatx4*>(&sm_o[i][mr][md + j]) * w[i];
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i) {
-        w[i] = rescale(sm_ml[i][mr][0], m);
-        lt = __builtin_fmaf(sm_ml[i][mr][1], w[i], lt);
-      }
-      float acc[W];
+    for (int e = 0; e < 4; ++e) acc[j + e] = x[e];
+  }
+  if (a.splits == 1) {
+    const float inv = inverse_sum(lt);
+    const int i = mr / a.group, h = hk * a.group + mr - i * a.group;
+    uint32_t out[W / 2];
 #pragma unroll
-      for (int j = 0; j < W; j += 4) {
-        floatx4 x = {0, 0, 0, 0};
+    for (int j = 0; j < W; j += 2) out[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
+    uint16_t* const dst = a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + md;
+    if constexpr (W == 8)
+      *reinterpret_cast<u32x4*>(dst) = u32x4{out[0], out[1], out[2], out[3]};
+    else
+      *reinterpret_cast<u32x2*>(dst) = u32x2{out[0], out[1]};
+  } else {
+    const int64_t item = ((static_cast<int64_t>(b) * a.hkv + hk) * a.splits + split) * kRowsBlock + mr;
+    const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.splits * kRowsBlock;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) x += *reinterpret_cast<const floatx4*>(&sm_o[i][mr][md + j]) * w[i];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j + e] = x[e];
-      }
-      const int i = row / a.group, h = hk * a.group + row - i * a.group;
-      if (a.splits == 1) {
-        const float inv = lt > 0.f ? 1.f / lt : lt == 0.f ? 1.f : lt;  // (nothing seen: O is 0, or NaN; lt NaN stays)
-        uint32_t out[W / 2];
-#pragma unroll
-        for (int j = 0; j < W; j += 2) out[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
-        uint16_t* const dst = a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + md;
-        if constexpr (W == 8)
-          *reinterpret_cast<u32x4*>(dst) = u32x4{out[0], out[1], out[2], out[3]};
-        else
-          *reinterpret_cast<u32x2*>(dst) = u32x2{out[0], out[1]};
-      } else {
-        const int64_t item = (((static_cast<int64_t>(b) * a.hkv + hk) * a.row_tiles + rt) * a.splits + split) * RB + 16 * nt + mr;
-        const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * RB;
-#pragma unroll
-        for (int j = 0; j < W; j += 4)
-          *reinterpret_cast<floatx4*>(a.part + item * D + md + j) = floatx4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
-        if (md == 0) {
-          a.part[items * D + item * 2] = m;
-          a.part[items * D + item * 2 + 1] = lt;
-        }
-      }
+    for (int j = 0; j < W; j += 4)
+      *reinterpret_cast<floatx4*>(a.part + item * D + md + j) = floatx4{acc[j], acc[j + 1], acc[j + 2], acc[j + 3]};
+    if (md == 0) {
+      a.part[items * D + item * 2] = m;
+      a.part[items * D + item * 2 + 1] = lt;
     }
   }
 }
@@ -636,22 +609,27 @@ __device__ __forceinline__ void read_v(u32x2 (&v0)[2][2], u32x2 (&v1)[2][2], uin
       : "memory");
 }
 
-template <int D, bool kCache, bool kMask>
-__global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
-  constexpr int RB = 128;
+template <int D, int NG, bool kCache, bool kMask>
+__global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
+  constexpr int NQ = kWaves / NG, RB = 32 * NQ;
   constexpr int KCH = D / 16;      // MFMA steps over head_dim
   constexpr int DBLK = D / 32;     // 32-dimension blocks of O^T
   constexpr int PCS = D / 8;       // 16-byte pieces of a row
   constexpr int ROWB = 2 * D;      // bytes of a row
   constexpr int CH = 32 * ROWB / 1024;   // 1 KB chunks of a tile's K or V
   constexpr int CPW = CH / kWaves;       // of them a wave loads (D = 64: one)
-  constexpr int TILEB = 2 * 32 * ROWB;   // K and V of a tile in LDS; a ring slot holds two tiles, a step's
+  constexpr int TILEB = 2 * 32 * ROWB;   // K and V of a tile in LDS; a ring slot holds NG tiles, a step's
+  constexpr int NS = kCache || NG > 1 ? 2 : 3;  // ring slots
   constexpr int OP = D + 8;              // pitch of O rows staged in LDS
-  constexpr int RING = 2 * 2 * TILEB, STAGE = kWaves * 32 * OP * 2;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[RING > STAGE ? RING : STAGE];
+  constexpr int RING = NS * NG * TILEB, STAGE = kWaves * 32 * OP * 2;
+  static_assert(NG == 1 || NG == 2 || NG == 4, "key groups");
+  constexpr int EXCH = NG > 1 ? kWaves * (DBLK * 4 + 1) * 1024 : 0;  // states that the key groups exchange
+  constexpr int LDS = RING > STAGE ? (RING > EXCH ? RING : EXCH) : (STAGE > EXCH ? STAGE : EXCH);
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[LDS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l32 = lane & 31, g = lane >> 5;
+  const int wq = wave % NQ, kg = wave / NQ;  // the wave's block of 32 rows, and its share of the tiles
 
   // work item: (batch, kv head, row tile, split), neighbours on one XCD (workgroup i runs on XCD i % 8)
   int id;
@@ -667,14 +645,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   const int hk = id % a.hkv, b = id / a.hkv;
 
   const int rows = a.sq * a.group;
-  const int row0 = rt * RB, rw0 = row0 + 32 * wave;
+  const int row0 = rt * RB, rw0 = row0 + 32 * wq;
   const Span sp = span_of<kCache>(a, b, row0, min(RB, rows - row0));
   const int use = splits_of(a.splits, sp.n);
   if (split >= use) return;
   const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
   const int n = static_cast<int>(static_cast<int64_t>(sp.n) * (split + 1) / use) - t0;
   auto tile_at = [&](int it) {
-    const int t = t0 + it;
+    const int t = t0 + min(it, n - 1);  // (past the end: the last one again)
     return t < sp.ns ? t : sp.w0 + (t - sp.ns);
   };
 
@@ -695,8 +673,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   // ---- tiles into LDS ----
   const uint16_t* const kb = kCache ? nullptr : a.k + b * a.k_sb + hk * a.k_sh;
   const uint16_t* const vb = kCache ? nullptr : a.v + b * a.v_sb + hk * a.v_sh;
-  auto swz_k = [](int r) { return r & (PCS - 1); };
-  auto swz_v = [](int r) { return 2 * (r & 3); };
+  auto swz_k = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
+  auto swz_v = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
   // this lane's rows and pieces of the wave's chunks
   int drow[CPW], dk[CPW], dv[CPW];
 #pragma unroll
@@ -807,10 +785,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   for (int db = 0; db < DBLK; ++db) oacc[db] = floatx16{};
   float m_ref = -__builtin_inff(), l = 0.f;
 
-  // the mask of a step's keys, a bit each (lanes 0 .. 31 load the first tile's, the others the second's, a step ahead)
+  // the mask of a tile's keys, a bit each (lanes 0 .. 31 load them, a step ahead)
   float mload = 1.f;
-  auto fetch_mask = [&](int ta, int tb) {
-    if constexpr (kMask) mload = a.mask[b * a.mask_sb + min((g ? tb : ta) * kTile + l32, a.limit - 1)];
+  auto fetch_mask = [&](int it) {
+    if constexpr (kMask) mload = a.mask[b * a.mask_sb + min(tile_at(it) * kTile + l32, a.limit - 1)];
   };
 
   // LDS addresses of this lane's part of the operands: piece g of row l32 of K; 8 bytes of row 4 g + (lane / 4) % 4 of
@@ -879,53 +857,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
                                                            oacc[db], 0, 0, 0);
       }
   };
-  // one matrix instruction, then its share of the 56 vector instructions (16 of them exponentials) of a tile's softmax
-  auto interleave = [&]() {
-#pragma unroll
-    for (int i = 0; i < KCH; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 40 / KCH, 0);
-      __builtin_amdgcn_sched_group_barrier(0x400, 16 / KCH, 0);
-    }
-  };
-
-  // Two tiles that the wave's queries see whole: the softmax of each between matrix instructions of the other.
-  auto compute2 = [&](int off) {
-    u32x4 kop[KCH], pa[2], pb[2];
-    u32x2 vop[DBLK][2][2];
-    floatx16 sa = floatx16{}, sb = floatx16{};
-    load_k(kop, off);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int c = 0; c < KCH; ++c)
-      sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], sa, 0, 0, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    load_k(kop, off + TILEB);
-    const float ma = top_of(sa);
-    if (__any(ma > m_ref + kMoveRef)) move_ref(ma);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int c = 0; c < KCH; ++c)
-      sb = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kop[c]), qf[c], sb, 0, 0, 0);
-    exp_all(sa);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(vop, off);
-    __builtin_amdgcn_sched_barrier(0);
-    const float mb = top_of(sb);
-    if (__any(mb > m_ref + kMoveRef)) sa *= move_ref(mb);
-    __builtin_amdgcn_sched_barrier(0);
-    pack(sa, pa);
-    pv(vop, pa);
-    exp_all(sb);
-    pack(sb, pb);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(vop, off + TILEB);
-    __builtin_amdgcn_sched_barrier(0);
-    pv(vop, pb);
-  };
-
   bool odd_v = false;  // (wave-uniform) some tile's V held infinities or NaN that not every query of the wave sees
 
   // Any tile.
@@ -954,17 +885,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
         const float sc = kCache && page < 0 ? __builtin_nanf("") : s[e];
         s[e] = vis & (1u << (8 * (e >> 2) + (e & 3))) ? sc : -__builtin_inff();
       }
-      bool dirty = false;
+      Largest big;
 #pragma unroll
       for (int db = 0; db < DBLK; ++db)
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            dirty |= nonfinite2(vop[db][s2][h][0]);
-            dirty |= nonfinite2(vop[db][s2][h][1]);
-          }
-      if (__any(dirty)) {
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) big.look(vop[db][s2][h][x]);
+      if (__any(big.nonfinite())) {
         // A key that a query does not see weighs 0, and 0 times an infinity or a NaN is a NaN: they go to the queries
         // that see them behind the loop, and count as zeros here.
         odd_v = true;
@@ -987,95 +917,62 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
   };
 
   if (n > 0) {
-    // Steps of two tiles in the two slots of the ring.  begin(st): step st's tiles are in LDS, the next ones on their way.
-    const int steps = (n + 1) / 2;
-    struct Step {
-      int k0, k1;      // first keys of the two tiles (an odd number of tiles: the last step has no second one)
-      int p0, p1;      // their pages, -1: missing (kCache)
-      uint64_t mask;   // of their 64 keys (kMask)
-      bool pair;       // a step for compute2
-    };
-    auto step = [&](int st, int k0, int k1, int p0, int p1, uint64_t mask) {
-      bool two = 2 * st + 1 < n;
-      two &= whole(k0);
-      two &= whole(k1);
-      two &= p0 >= 0;
-      two &= p1 >= 0;
-      two &= mask == ~uint64_t{0};
-      return Step{k0, k1, p0, p1, mask, two};
-    };
-    auto run = [&](auto begin) {
-      int st = 0;
-      Step x = begin(0);
-      // (two loops, so that the state does not change registers at every step)
-      while (st < steps) {
-        while (st < steps && !x.pair) {
-          const int off = (st & 1) * 2 * TILEB;
-          compute(x.k0, off, x.p0, static_cast<uint32_t>(x.mask));
-          if (2 * st + 1 < n) compute(x.k1, off + TILEB, x.p1, static_cast<uint32_t>(x.mask >> 32));
-          if (++st < steps) x = begin(st);
-        }
-        while (st < steps && x.pair) {
-          compute2((st & 1) * 2 * TILEB);
-          if (++st < steps) x = begin(st);
-        }
-      }
-    };
+    // step st brings the tiles st NG .. + NG - 1, of which key group kg takes st NG + kg
+    const int steps = (n + NG - 1) / NG;
     if constexpr (kCache) {
       load_ids(0);
-      u32x4 codes[2];
-      uint32_t scales[2];
-      int page[2], page_next[2] = {-1, -1};
-      auto fetch2 = [&](int st, int (&pg)[2]) {
+      u32x4 codes[NG];
+      uint32_t scales[NG];
+      int own = -1, own_next = -1;  // the page of this wave's tile
+      auto fetch_step = [&](int st) {
+        int mine = -1;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          pg[x] = 2 * st + x < n ? page_of(2 * st + x) : -1;
-          fetch(pg[x], 2 * st + x, codes[x], scales[x]);
+        for (int x = 0; x < NG; ++x) {
+          const int page = st * NG + x < n ? page_of(st * NG + x) : -1;
+          fetch(page, st * NG + x, codes[x], scales[x]);
+          mine = x == kg ? page : mine;
         }
+        return mine;
       };
-      auto store2 = [&](int slot) {
+      auto store_step = [&](int slot) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) store((2 * slot + x) * TILEB, codes[x], scales[x]);
+        for (int x = 0; x < NG; ++x) store((slot * NG + x) * TILEB, codes[x], scales[x]);
       };
-      fetch2(0, page);
-      store2(0);
-      if (steps > 1) fetch2(1, page_next);
-      run([&](int st) {
+      own = fetch_step(0);
+      store_step(0);
+      if (steps > 1) own_next = fetch_step(1);
+      for (int st = 0; st < steps; ++st) {
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int p0 = page[0], p1 = page[1];
-        if (st + 1 < steps) store2((st + 1) & 1);
-        page[0] = page_next[0], page[1] = page_next[1];
-        if (st + 2 < steps) fetch2(st + 2, page_next);
-        return step(st, tile_at(2 * st) * kTile, tile_at(2 * st + 1) * kTile, p0, p1, ~uint64_t{0});
-      });
+        const int page = own;
+        own = own_next;
+        if (st + 1 < steps) store_step((st + 1) & 1);
+        if (st + 2 < steps) own_next = fetch_step(st + 2);
+        if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, ((st & 1) * NG + kg) * TILEB, page, ~0u);
+      }
     } else {
-      // tiles of this step and the next one (past the end: the last one again)
-      const int t_last = tile_at(n - 1);
-      auto next = [&](int t) { return t == t_last ? t : t + 1 == sp.ns ? sp.w0 : t + 1; };
-      int ta = tile_at(0), tb = next(ta);
-      fetch_mask(ta, tb);
-      dma(ta, 0);
-      dma(tb, TILEB);
-      run([&](int st) {
-        vm_wait_barrier<0>();  // the step's tiles are in LDS, the other slot is free
-        uint64_t mask = ~uint64_t{0};
-        if constexpr (kMask) mask = __ballot(mload != 0.f);
-        const Step x = step(st, ta * kTile, tb * kTile, 0, 0, mask);
-        ta = next(tb), tb = next(ta);
-        if (st + 1 < steps) {
-          const int to = ((st + 1) & 1) * 2 * TILEB;
-          fetch_mask(ta, tb);
-          dma(ta, to);
-          dma(tb, to + TILEB);
-        }
-        return x;
-      });
+      auto dma_step = [&](int st, int slot) {
+#pragma unroll
+        for (int x = 0; x < NG; ++x) dma(tile_at(st * NG + x), (slot * NG + x) * TILEB);
+      };
+      fetch_mask(kg);
+#pragma unroll
+      for (int x = 0; x < NS - 1; ++x) dma_step(x, x);
+      int slot = 0;
+      for (int st = 0; st < steps; ++st) {
+        vm_wait_barrier<(NS - 2) * NG * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
+        uint32_t mask = ~0u;
+        if constexpr (kMask) mask = static_cast<uint32_t>(__ballot(mload != 0.f));
+        fetch_mask((st + 1) * NG + kg);
+        dma_step(st + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+        if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, (slot * NG + kg) * TILEB, 0, mask);
+        slot = slot + 1 == NS ? 0 : slot + 1;
+      }
     }
   }
   vm_wait_barrier<0>();  // every wave has read its last tile, no load into LDS is in flight
 
   if (__builtin_expect(odd_v, 0)) {
-    for (int it = 0; it < n; ++it) {
+    for (int it = kg; it < n; it += NG) {
       const int k0 = tile_at(it) * kTile;
       if (skipped(k0)) continue;
       uint32_t mbits = ~0u;
@@ -1107,28 +1004,87 @@ __global__ __launch_bounds__(64 * kWaves, D == 128 ? 2 : 3) void tile_attn_kerne
     }
   }
 
-  const float lt = pair_sum(l);
-  if (a.splits > 1) {
-    if (rw0 + l32 < rows) {
-      const int64_t item = (((static_cast<int64_t>(b) * a.hkv + hk) * a.row_tiles + rt) * a.splits + split) * RB + 32 * wave + l32;
-      const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * RB;
+  float lt = pair_sum(l);
+  const int row_at = rw0 + l32;
+  if constexpr (NG > 1) {
+    // The key groups of a row block exchange their states; group kg finishes the blocks kg, kg + NG, ... of O^T.
+    floatx4* const ex = reinterpret_cast<floatx4*>(ring);
+    constexpr int PER = (DBLK * 4 + 1) * 64;
+    floatx4* const mine = ex + wave * PER;
 #pragma unroll
-      for (int db = 0; db < DBLK; ++db)
+    for (int db = 0; db < DBLK; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        mine[(db * 4 + q4) * 64 + lane] = floatx4{oacc[db][4 * q4], oacc[db][4 * q4 + 1], oacc[db][4 * q4 + 2], oacc[db][4 * q4 + 3]};
+    mine[DBLK * 4 * 64 + lane] = floatx4{m_ref, lt, 0.f, 0.f};
+    __syncthreads();
+    float mg[NG], wg[NG], m = -__builtin_inff();
+    lt = 0.f;
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      mg[x] = ex[(wq + NQ * x) * PER + DBLK * 4 * 64 + lane][0];
+      m = fmaxf(m, mg[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < NG; ++x) {
+      wg[x] = rescale(mg[x], m);
+      lt = __builtin_fmaf(ex[(wq + NQ * x) * PER + DBLK * 4 * 64 + lane][1], wg[x], lt);
+    }
+    m_ref = m;
+#pragma unroll
+    for (int y = 0; y < (DBLK + NG - 1) / NG; ++y) {
+      const int db = kg + y * NG;
+      if (db < DBLK) {
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4) {
-          floatx4 x = {oacc[db][4 * q4], oacc[db][4 * q4 + 1], oacc[db][4 * q4 + 2], oacc[db][4 * q4 + 3]};
-          if (kCache && pos >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-          *reinterpret_cast<floatx4*>(a.part + item * D + 32 * db + 8 * q4 + 4 * g) = x;
+          floatx4 x = {0, 0, 0, 0};
+#pragma unroll
+          for (int z = 0; z < NG; ++z) x += ex[(wq + NQ * z) * PER + (db * 4 + q4) * 64 + lane] * wg[z];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) oacc[y][4 * q4 + e] = x[e];
         }
-      if (g == 0) {
+      }
+    }
+  }
+  constexpr int MINE = (DBLK + NG - 1) / NG;  // blocks of O^T that this wave finishes, the y-th at kg + y NG
+  if (a.splits > 1) {
+    if (row_at < rows) {
+      const int64_t item = (((static_cast<int64_t>(b) * a.hkv + hk) * a.row_tiles + rt) * a.splits + split) * RB + 32 * wq + l32;
+      const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * RB;
+#pragma unroll
+      for (int y = 0; y < MINE; ++y)
+        if (kg + y * NG < DBLK) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            floatx4 x = {oacc[y][4 * q4], oacc[y][4 * q4 + 1], oacc[y][4 * q4 + 2], oacc[y][4 * q4 + 3]};
+            if (kCache && pos >= a.limit) x = floatx4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            *reinterpret_cast<floatx4*>(a.part + item * D + 32 * (kg + y * NG) + 8 * q4 + 4 * g) = x;
+          }
+        }
+      if (g == 0 && kg == 0) {
         a.part[items * D + item * 2] = m_ref;
         a.part[items * D + item * 2 + 1] = lt;
       }
     }
     return;
   }
-  float inv = lt > 0.f ? 1.f / lt : lt == 0.f ? 1.f : lt;
+  float inv = inverse_sum(lt);
   if (kCache && pos >= a.limit) inv = __builtin_nanf("");  // (sees slots that nobody can read)
+  if constexpr (NG > 1) {
+    if (row_at < rows) {
+      uint16_t* const dst = a.o + b * a.o_sb + qi * a.o_ss + qh * a.o_sh + 4 * g;
+#pragma unroll
+      for (int y = 0; y < MINE; ++y)
+        if (kg + y * NG < DBLK) {
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<u32x2*>(dst + 32 * (kg + y * NG) + 8 * q4) =
+                u32x2{pack_bf16x2(oacc[y][4 * q4] * inv, oacc[y][4 * q4 + 1] * inv),
+                      pack_bf16x2(oacc[y][4 * q4 + 2] * inv, oacc[y][4 * q4 + 3] * inv)};
+        }
+    }
+    return;
+  }
   uint16_t* const st = reinterpret_cast<uint16_t*>(ring) + wave * (32 * OP);
 #pragma unroll
   for (int db = 0; db < DBLK; ++db)
@@ -1202,7 +1158,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb
   __syncthreads();
   const int d = static_cast<int>(threadIdx.x);
   if (d >= D / 2) return;
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 1.f : l;
+  const float inv = inverse_sum(l);
   float x0 = 0.f, x1 = 0.f;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
@@ -1218,9 +1174,11 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb
 // ---------------------------------------------------------------------------
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+constexpr int64_t kWide = 400, kHalf = 256;  // workgroups from which on they take 128 rows, 64 rows
+
 // How a call is cut up; depends on sizes alone.
 struct Plan {
-  int rb, row_tiles, splits;  // rows of a workgroup: 16, 32, 64 (rows_attn_kernel) or 128 (tile_attn_kernel)
+  int rb, row_tiles, splits;  // rows of a workgroup: 16 (rows_attn_kernel), 32, 64 or 128 (tile_attn_kernel)
   int64_t items;  // row blocks times splits
   int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * rb * (head_dim + 2) * 4 : 0; }
 };
@@ -1233,15 +1191,18 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     return false;
   const int64_t group = q_heads / kv_heads, rows = seq_q * group;
   if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
-  p.rb = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
-  const int64_t rb = p.rb;
-  p.row_tiles = static_cast<int>(rows == 0 ? 1 : (rows + rb - 1) / rb);
-  const int64_t blocks = std::max<int64_t>(1, batch * kv_heads * p.row_tiles);
+  const int64_t heads = std::max<int64_t>(1, batch * kv_heads);
+  if (rows <= kRowsBlock)
+    p.rb = kRowsBlock;
+  else
+    p.rb = heads * ((rows + 127) / 128) >= kWide ? 128 : heads * ((rows + 63) / 64) >= kHalf ? 64 : 32;
+  p.row_tiles = static_cast<int>(rows == 0 ? 1 : (rows + p.rb - 1) / p.rb);
+  const int64_t blocks = heads * p.row_tiles;
   // tiles of the longest row block
-  const int64_t span = std::min(limit, std::min(window, limit) + rb / std::max<int64_t>(1, group) + 1);
+  const int64_t span = std::min(limit, std::min(window, limit) + p.rb / std::max<int64_t>(1, group) + 1);
   const int64_t tiles = std::min((limit + kTile - 1) / kTile,
                                  (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
-  const int64_t want = std::max<int64_t>(1, (p.rb >= 64 ? 256 : 512) / blocks);
+  const int64_t want = std::max<int64_t>(1, (p.rb == kRowsBlock ? 512 : 256) / blocks);
   p.splits = static_cast<int>(std::min<int64_t>({64, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
   p.items = blocks * p.splits;
   return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
@@ -1271,22 +1232,27 @@ void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* 
   a.part = static_cast<float*>(workspace);
 }
 
-template <int D, bool kCache>
-hipError_t launch_rows(const StreamArgs& a, const Plan& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.items)), block(64 * kWaves);
-  if (p.rb == 128) {
-    if constexpr (kCache)
-      hipLaunchKernelGGL((tile_attn_kernel<D, true, false>), grid, block, 0, stream, a);
-    else if (a.mask)
-      hipLaunchKernelGGL((tile_attn_kernel<D, false, true>), grid, block, 0, stream, a);
-    else
-      hipLaunchKernelGGL((tile_attn_kernel<D, false, false>), grid, block, 0, stream, a);
-  } else if (p.rb == 16)
-    hipLaunchKernelGGL((rows_attn_kernel<D, 1, kCache>), grid, block, 0, stream, a);
-  else if (p.rb == 32)
-    hipLaunchKernelGGL((rows_attn_kernel<D, 2, kCache>), grid, block, 0, stream, a);
+template <int D, int NG, bool kCache>
+void launch_tiles(const StreamArgs& a, dim3 grid, hipStream_t stream) {
+  if constexpr (kCache)
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, true, false>), grid, dim3(64 * kWaves), 0, stream, a);
+  else if (a.mask)
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, true>), grid, dim3(64 * kWaves), 0, stream, a);
   else
-    hipLaunchKernelGGL((rows_attn_kernel<D, 4, kCache>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, false>), grid, dim3(64 * kWaves), 0, stream, a);
+}
+
+template <int D, bool kCache>
+hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.items)), block(64 * kWaves);
+  if (p.rb == kRowsBlock)
+    hipLaunchKernelGGL((rows_attn_kernel<D, kCache>), grid, block, 0, stream, a);
+  else if (p.rb == 32)
+    launch_tiles<D, 4, kCache>(a, grid, stream);
+  else if (p.rb == 64)
+    launch_tiles<D, 2, kCache>(a, grid, stream);
+  else
+    launch_tiles<D, 1, kCache>(a, grid, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>(a.batch * a.hq * a.sq)), block, 0, stream, a,
@@ -1339,7 +1305,7 @@ extern "C" hipError_t rldx_window_attention_bf16(const void* q, const int64_t* q
   a.v_sb = v_strides[0], a.v_ss = v_strides[1], a.v_sh = v_strides[2];
   a.mask = key_mask;
   a.mask_sb = key_mask_batch_stride;
-  return head_dim == 128 ? launch_rows<128, false>(a, p, stream) : launch_rows<64, false>(a, p, stream);
+  return head_dim == 128 ? launch<128, false>(a, p, stream) : launch<64, false>(a, p, stream);
 }
 
 extern "C" int64_t rldx_kv4_attention_workspace_bytes(int64_t batch, int64_t q_heads, int64_t kv_heads,
@@ -1379,5 +1345,5 @@ extern "C" hipError_t rldx_kv4_attention_bf16(const void* q, const int64_t* q_st
   a.table_sb = cache->page_table_stride;
   a.starts = starts;
   a.counts = counts;
-  return cache->head_dim == 128 ? launch_rows<128, true>(a, p, stream) : launch_rows<64, true>(a, p, stream);
+  return cache->head_dim == 128 ? launch<128, true>(a, p, stream) : launch<64, true>(a, p, stream);
 }
