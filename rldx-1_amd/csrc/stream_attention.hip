@@ -36,6 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = kv4::kTile;
 constexpr int kWaves = 4;
 constexpr int kRowsBlock = 16;  // rows of a rows_attn_kernel workgroup
+constexpr int kMaxSplits = 64;
 constexpr int kMaxSlots = 1 << 30;
 constexpr float kMoveRef = 5.f;  // log2 units: the softmax reference moves when a score exceeds it by 2^5
 
@@ -148,14 +149,14 @@ __device__ __forceinline__ bf16x8 dequant8(uint32_t c, float s) {
 
 // (The pairs are opaque to the compiler in these, or it works them out ahead for every tile, and keeps registers for
 // them, though only a few tiles come here.)
-// The largest magnitude of bf16 values, whose bits order as they do: an infinity or a NaN is 0x7f80 or more.
-struct Largest {
-  u16x2 m = {0, 0};
+// Whether any of the bf16 values looked at is an infinity or a NaN: 0 times it is a NaN.
+struct Finite {
+  float sum = 0.f;
   __device__ __forceinline__ void look(uint32_t w) {
     asm volatile("" : "+v"(w));
-    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w & 0x7fff7fffu));
+    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{0, 0}, sum, false);
   }
-  __device__ __forceinline__ bool nonfinite() const { return (m[0] >= 0x7f80) | (m[1] >= 0x7f80); }
+  __device__ __forceinline__ bool broken() const { return sum != sum; }
 };
 __device__ __forceinline__ uint32_t finite2(uint32_t w) {  // with zeros in the place of what is not
   asm volatile("" : "+v"(w));
@@ -174,6 +175,11 @@ __device__ __forceinline__ float mark_value(int kind) {
 }
 
 // The keys 0 .. 31 of a tile that a query sees, a bit each: k0 <= p, and k0 > p - window or k0 < sinks.
+// s where bit c is set, else -inf
+__device__ __forceinline__ float seen_or_none(float s, uint32_t bits, int c) {
+  const uint32_t m = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), c, 1));
+  return __builtin_bit_cast(float, (m & __builtin_bit_cast(uint32_t, s)) | (~m & 0xff800000u));
+}
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 __device__ __forceinline__ uint32_t visible_bits(int k0, int p, int window, int sinks) {
   return below(p + 1 - k0) & (~below(p + 1 - window - k0) | below(sinks - k0));
@@ -364,9 +370,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float sc = kCache && page < 0 ? __builtin_nanf("") : s[kt][r];
-          s[kt][r] = vis & (1u << (16 * kt + r)) ? sc : -__builtin_inff();
+          s[kt][r] = seen_or_none(sc, vis, 16 * kt + r);
         }
-      Largest big;
+      Finite v;
       bool dirty = false;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -376,11 +382,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
 #pragma unroll
           for (int j = 0; j < W / 2; ++j) {
             const uint32_t w = raw.v[i][j];
-            big.look(w);
+            v.look(w);
           }
         }
       }
-      odd_v = __any(dirty || big.nonfinite());
+      odd_v = __any(dirty || v.broken());
     }
     // ---- softmax ----
     float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
@@ -610,7 +616,7 @@ __device__ __forceinline__ void read_v(u32x2 (&v0)[2][2], u32x2 (&v1)[2][2], uin
 }
 
 template <int D, int NG, bool kCache, bool kMask>
-__global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
+__global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && (kCache || kMask)) ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
   constexpr int NQ = kWaves / NG, RB = 32 * NQ;
   constexpr int KCH = D / 16;      // MFMA steps over head_dim
   constexpr int DBLK = D / 32;     // 32-dimension blocks of O^T
@@ -640,7 +646,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
   }
   const int split = id % a.splits;
   id /= a.splits;
-  const int rt = id % a.row_tiles;
+  const int rt = a.row_tiles - 1 - id % a.row_tiles;  // (the last rows first: they may have the longest spans)
   id /= a.row_tiles;
   const int hk = id % a.hkv, b = id / a.hkv;
 
@@ -683,13 +689,17 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
     dk[c] = drow[c] * static_cast<int>(a.k_ss * 2) + ((lane % PCS) ^ swz_k(drow[c])) * 16;
     dv[c] = drow[c] * static_cast<int>(a.v_ss * 2) + ((lane % PCS) ^ swz_v(drow[c])) * 16;
   }
-  auto dma = [&](int tile, int off) {  // off: of the tile's place in LDS
-    const int k0 = tile * kTile;
-    // (rows of less than 2^25 bytes: the step from tile to tile has 31 bits)
-    const uint8_t* const kt = reinterpret_cast<const uint8_t*>(kb) +
-                              static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.k_ss * (2 * kTile));
-    const uint8_t* const vt = reinterpret_cast<const uint8_t*>(vb) +
-                              static_cast<uint64_t>(static_cast<uint32_t>(tile)) * static_cast<uint32_t>(a.v_ss * (2 * kTile));
+  // the next tile that the workgroup brings: its first key and its rows (past the end: the last one again)
+  const int64_t kstep = a.k_ss * (2 * kTile), vstep = a.v_ss * (2 * kTile);
+  const uint8_t *kt = nullptr, *vt = nullptr;
+  int d_it = 0, d_tile = 0;
+  auto dma_seek = [&](int tile) {
+    d_tile = tile;
+    kt = reinterpret_cast<const uint8_t*>(kb) + tile * kstep;
+    vt = reinterpret_cast<const uint8_t*>(vb) + tile * vstep;
+  };
+  auto dma = [&](int off) {
+    const int k0 = d_tile * kTile;
     uint8_t* const to = ring + off + wave * 1024;
     int ok[CPW], ov[CPW];
 #pragma unroll
@@ -706,6 +716,15 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
     for (int c = 0; c < CPW; ++c) load_lds16(kt, to + kWaves * c * 1024, ok[c]);
 #pragma unroll
     for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + kWaves * c * 1024, ov[c]);
+    if (++d_it < n) {
+      if (d_tile + 1 == sp.ns) {
+        dma_seek(sp.w0);
+      } else {
+        ++d_tile;
+        kt += kstep;
+        vt += vstep;
+      }
+    }
   };
   // page ids of 64 tiles, one a lane
   int ids = -1, ids_base = 0;
@@ -783,7 +802,9 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
   floatx16 oacc[DBLK];
 #pragma unroll
   for (int db = 0; db < DBLK; ++db) oacc[db] = floatx16{};
-  float m_ref = -__builtin_inff(), l = 0.f;
+  // The softmax reference m_ref (log2 units), the score beyond which it moves, and -m_ref for the exponent's argument
+  // (0 as long as there is none: p = exp2(-inf) = 0)
+  float m_ref = -__builtin_inff(), m_move = -__builtin_inff(), m_neg = 0.f, l = 0.f;
 
   // the mask of a tile's keys, a bit each (lanes 0 .. 31 load them, a step ahead)
   float mload = 1.f;
@@ -820,23 +841,24 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
     float mt = s[0];
 #pragma unroll
     for (int e = 1; e < 16; ++e) mt = fmaxf(mt, s[e]);
-    return mt * a.scale_log2;
+    return mt;
   };
+  const float inv_scale = 1.f / a.scale_log2;
   auto move_ref = [&](float mt) {
-    const float nr = fmaxf(m_ref, pair_max(mt));
+    const float nr = fmaxf(m_ref, pair_max(mt) * a.scale_log2);
     const float al = rescale(m_ref, nr);
     m_ref = nr;
+    m_move = (nr + kMoveRef) * inv_scale;
+    m_neg = nr == -__builtin_inff() ? 0.f : -nr;
     l *= al;
 #pragma unroll
     for (int db = 0; db < DBLK; ++db) oacc[db] *= al;
-    return al;
   };
   auto exp_all = [&](floatx16& s) {
-    const float nm = m_ref == -__builtin_inff() ? 0.f : -m_ref;
     float ps = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, nm));
+      s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], a.scale_log2, m_neg));
       ps += s[e];
     }
     l += ps;
@@ -860,9 +882,16 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
   bool odd_v = false;  // (wave-uniform) some tile's V held infinities or NaN that not every query of the wave sees
 
   // Any tile.
+  // Tiles that start at w_lo .. w_lo + w_len - 1 lie whole in the windows of all of the wave's queries.
+  const int w_lo = max(pw1 - a.window + 1, 0), w_len = all_rows ? max(pw0 - kTile + 2 - w_lo, 0) : 0;
   auto compute = [&](int k0, int off, int page, uint32_t mbits) {
-    if (skipped(k0)) return;
+    bool full = static_cast<unsigned>(k0 - w_lo) < static_cast<unsigned>(w_len);
+    if (!full) {
+      if (skipped(k0)) return;
+      full = whole(k0);  // (the sinks' tiles)
+    }
     if (kMask && mbits == 0) return;
+    full = full && page >= 0 && mbits == 0xffffffffu;
     floatx16 s = floatx16{};
     u32x2 vop[DBLK][2][2];
     {
@@ -877,15 +906,14 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
     load_v(vop, off);
     __builtin_amdgcn_sched_barrier(0);
     // ---- visibility ----
-    const bool full = whole(k0) && page >= 0 && mbits == 0xffffffffu;
     if (!full) {
       const uint32_t vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const float sc = kCache && page < 0 ? __builtin_nanf("") : s[e];
-        s[e] = vis & (1u << (8 * (e >> 2) + (e & 3))) ? sc : -__builtin_inff();
+        s[e] = seen_or_none(sc, vis, 8 * (e >> 2) + (e & 3));
       }
-      Largest big;
+      Finite v;
 #pragma unroll
       for (int db = 0; db < DBLK; ++db)
 #pragma unroll
@@ -893,8 +921,8 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) big.look(vop[db][s2][h][x]);
-      if (__any(big.nonfinite())) {
+            for (int x = 0; x < 2; ++x) v.look(vop[db][s2][h][x]);
+      if (__any(v.broken())) {
         // A key that a query does not see weighs 0, and 0 times an infinity or a NaN is a NaN: they go to the queries
         // that see them behind the loop, and count as zeros here.
         odd_v = true;
@@ -909,7 +937,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
       }
     }
     const float mt = top_of(s);
-    if (__any(mt > m_ref + kMoveRef)) move_ref(mt);
+    if (__any(mt > m_move)) move_ref(mt);
     u32x4 pk[2];
     exp_all(s);
     pack(s, pk);
@@ -950,20 +978,21 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
         if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, ((st & 1) * NG + kg) * TILEB, page, ~0u);
       }
     } else {
-      auto dma_step = [&](int st, int slot) {
+      auto dma_step = [&](int slot) {
 #pragma unroll
-        for (int x = 0; x < NG; ++x) dma(tile_at(st * NG + x), (slot * NG + x) * TILEB);
+        for (int x = 0; x < NG; ++x) dma((slot * NG + x) * TILEB);
       };
       fetch_mask(kg);
+      dma_seek(tile_at(0));
 #pragma unroll
-      for (int x = 0; x < NS - 1; ++x) dma_step(x, x);
+      for (int x = 0; x < NS - 1; ++x) dma_step(x);
       int slot = 0;
       for (int st = 0; st < steps; ++st) {
         vm_wait_barrier<(NS - 2) * NG * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
         uint32_t mask = ~0u;
         if constexpr (kMask) mask = static_cast<uint32_t>(__ballot(mload != 0.f));
         fetch_mask((st + 1) * NG + kg);
-        dma_step(st + NS - 1, slot == 0 ? NS - 1 : slot - 1);
+        dma_step(slot == 0 ? NS - 1 : slot - 1);
         if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, (slot * NG + kg) * TILEB, 0, mask);
         slot = slot + 1 == NS ? 0 : slot + 1;
       }
@@ -1105,76 +1134,85 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || kCache ? 2 : 
   }
 }
 
-// O of a query row from the partial states of its splits: wave w adds up splits w, w + 4, ...
+// O of the query rows from the partial states of their splits: `per` waves (1 up to 16 splits, else 4) to a row, wave w
+// of them adds up splits w, w + per, ... .  Every state is loaded before anything is known about its use: one round trip
+// through memory, whichever of the splits had tiles.
 template <int D, bool kCache>
-__global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb) {
+__global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb, int per) {
   constexpr int E = D / 64;  // dimensions per lane
+  constexpr int U = kMaxSplits / kWaves;
   __shared__ float sm[kWaves][D];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-  const int rows = a.sq * a.group;
-  int id = static_cast<int>(blockIdx.x);
-  const int row = id % rows;
-  id /= rows;  // b hkv + hk
-  const int b = id / a.hkv, hk = id - b * a.hkv;
+  const int rows = a.sq * a.group, share = wave % per;
+  const int at = static_cast<int>(blockIdx.x) * (kWaves / per) + wave / per;
+  if (at >= a.batch * a.hkv * rows) return;  // (one wave to a row: no barrier follows)
+  const int bh = at / rows, row = at - bh * rows;
+  const int b = bh / a.hkv, hk = bh - b * a.hkv;
   const int rt = row / rb;
-  const Span sp = span_of<kCache>(a, b, rt * rb, min(rb, rows - rt * rb));
-  const int use = splits_of(a.splits, sp.n);  // <= 64
-  const int64_t first = (static_cast<int64_t>(id) * a.row_tiles + rt) * a.splits * rb + (row - rt * rb);
+  const int64_t first = (static_cast<int64_t>(bh) * a.row_tiles + rt) * a.splits * rb + (row - rt * rb);
   const int64_t items = static_cast<int64_t>(a.batch) * a.hkv * a.row_tiles * a.splits * rb;
-  float m = -__builtin_inff(), l = 0.f;
-  if (lane < use) {
-    const float* const ml = a.part + items * D + (first + static_cast<int64_t>(lane) * rb) * 2;
-    m = ml[0];
-    l = ml[1];
-  }
-  float top = m;
+  float x[U][E] = {};
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-  const float w = rescale(m, top);
-  l *= w;
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
-  float acc[E] = {};
-  for (int s0 = wave; s0 < use; s0 += 8 * kWaves) {
-    float x[8][E];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int s = min(s0 + u * kWaves, use - 1);
+  for (int u = 0; u < U; ++u) {
+    const int s = share + per * u;
+    if (s < a.splits) {
       const float* const src = a.part + (first + static_cast<int64_t>(s) * rb) * D + lane * E;
 #pragma unroll
       for (int e = 0; e < E; ++e) x[u][e] = src[e];
     }
+  }
+  float m = -__builtin_inff(), l = 0.f;
+  if (lane < a.splits) {
+    const float* const ml = a.part + items * D + (first + static_cast<int64_t>(lane) * rb) * 2;
+    m = ml[0];
+    l = ml[1];
+  }
+  const Span sp = span_of<kCache>(a, b, rt * rb, min(rb, rows - rt * rb));
+  const int use = splits_of(a.splits, sp.n);
+  m = lane < use ? m : -__builtin_inff();
+  float top = m;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (s0 + u * kWaves >= use) break;
-      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s0 + u * kWaves));
+  for (int y = 1; y < 64; y *= 2) top = fmaxf(top, __shfl_xor(top, y));
+  const float w = rescale(m, top);
+  l = lane < use ? l * w : 0.f;
+#pragma unroll
+  for (int y = 1; y < 64; y *= 2) l += __shfl_xor(l, y);
+  float acc[E] = {};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int s = share + per * u;
+    if (s < use) {
+      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s));
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = __builtin_fmaf(x[u][e], ws, acc[e]);
     }
   }
+  if (per > 1) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm[wave][lane * E + e] = acc[e];
-  __syncthreads();
-  const int d = static_cast<int>(threadIdx.x);
-  if (d >= D / 2) return;
-  const float inv = inverse_sum(l);
-  float x0 = 0.f, x1 = 0.f;
+    for (int e = 0; e < E; ++e) sm[wave][lane * E + e] = acc[e];
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    x0 += sm[i][2 * d];
-    x1 += sm[i][2 * d + 1];
+    for (int e = 0; e < E; ++e) {
+      acc[e] = sm[0][lane * E + e];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) acc[e] += sm[i][lane * E + e];
+    }
   }
+  const float inv = inverse_sum(l);
   const int i = row / a.group, h = hk * a.group + row - i * a.group;
-  *reinterpret_cast<uint32_t*>(a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + 2 * d) = pack_bf16x2(x0 * inv, x1 * inv);
+  uint16_t* const dst = a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + lane * E;
+  if constexpr (E == 2)
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else
+    *dst = f32_to_bf16_bits(acc[0] * inv);
 }
 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
-constexpr int64_t kWide = 400, kHalf = 256;  // workgroups from which on they take 128 rows, 64 rows
 
 // How a call is cut up; depends on sizes alone.
 struct Plan {
@@ -1185,25 +1223,32 @@ struct Plan {
 
 // limit: readable keys.  false: sizes that the kernels do not take.
 bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t limit, int64_t head_dim,
-             int64_t window, int64_t sinks) {
+             int64_t window, int64_t sinks, bool cache) {
   if ((head_dim != 64 && head_dim != 128) || batch < 0 || q_heads < 0 || kv_heads <= 0 || q_heads % kv_heads ||
       seq_q < 0 || limit < 0 || limit > kMaxSlots || window < 1 || sinks < 0 || batch > 65535 || q_heads > 65535)
     return false;
   const int64_t group = q_heads / kv_heads, rows = seq_q * group;
   if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
   const int64_t heads = std::max<int64_t>(1, batch * kv_heads);
+  const auto row_tiles = [&](int64_t rb) { return (rows + rb - 1) / rb; };
+  // The smallest row blocks whose workgroups run all at once (per CU, by LDS and registers: 1 and 2 of 32 and 64 rows for
+  // head_dim 128, 2 and 4 for 64), else 128 rows.  Over the cache every block turns the codes into values again,
+  // so it takes 128 rows and splits the keys from 65 rows on.
+  const int64_t cus = 256, per_cu = head_dim == 128 ? 1 : 2;
   if (rows <= kRowsBlock)
     p.rb = kRowsBlock;
+  else if (cache)
+    p.rb = rows <= 64 ? 32 : 128;
   else
-    p.rb = heads * ((rows + 127) / 128) >= kWide ? 128 : heads * ((rows + 63) / 64) >= kHalf ? 64 : 32;
-  p.row_tiles = static_cast<int>(rows == 0 ? 1 : (rows + p.rb - 1) / p.rb);
+    p.rb = heads * row_tiles(32) <= per_cu * cus ? 32 : heads * row_tiles(64) <= 2 * per_cu * cus ? 64 : 128;
+  p.row_tiles = static_cast<int>(rows == 0 ? 1 : row_tiles(p.rb));
   const int64_t blocks = heads * p.row_tiles;
   // tiles of the longest row block
   const int64_t span = std::min(limit, std::min(window, limit) + p.rb / std::max<int64_t>(1, group) + 1);
   const int64_t tiles = std::min((limit + kTile - 1) / kTile,
                                  (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
-  const int64_t want = std::max<int64_t>(1, (p.rb == kRowsBlock ? 512 : 256) / blocks);
-  p.splits = static_cast<int>(std::min<int64_t>({64, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
+  const int64_t want = std::max<int64_t>(1, (p.rb == kRowsBlock ? 2 : 1) * cus / blocks);
+  p.splits = static_cast<int>(std::min<int64_t>({kMaxSplits, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
   p.items = blocks * p.splits;
   return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
 }
@@ -1255,8 +1300,10 @@ hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
     launch_tiles<D, 1, kCache>(a, grid, stream);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>(a.batch * a.hq * a.sq)), block, 0, stream, a,
-                     p.rb);
+  const int per = p.splits <= kMaxSplits / kWaves ? 1 : kWaves;  // waves to a row
+  const int64_t out_rows = static_cast<int64_t>(a.batch) * a.hq * a.sq;
+  hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>((out_rows * per + kWaves - 1) / kWaves)), block, 0,
+                     stream, a, p.rb, per);
   return hipGetLastError();
 }
 
@@ -1274,7 +1321,7 @@ extern "C" int64_t rldx_window_attention_workspace_bytes(int64_t batch, int64_t 
                                                          int64_t seq_q, int64_t seq_k, int64_t head_dim,
                                                          int64_t window, int64_t sinks) {
   Plan p;
-  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks)) return -1;
+  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks, false)) return -1;
   return p.workspace(head_dim);
 }
 
@@ -1286,7 +1333,7 @@ extern "C" hipError_t rldx_window_attention_bf16(const void* q, const int64_t* q
                                                  int64_t key_mask_batch_stride, float scale, void* workspace,
                                                  int64_t workspace_bytes, hipStream_t stream) {
   Plan p;
-  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks) ||
+  if (seq_q > seq_k || !plan_of(p, batch, q_heads, kv_heads, seq_q, seq_k, head_dim, window, sinks, false) ||
       !common_ok(q, q_strides, o, o_strides, scale) || !strides_ok(k_strides) || !strides_ok(v_strides) || !a16(k) ||
       !a16(v) || reinterpret_cast<uintptr_t>(key_mask) % 4)
     return hipErrorInvalidValue;
@@ -1313,7 +1360,7 @@ extern "C" int64_t rldx_kv4_attention_workspace_bytes(int64_t batch, int64_t q_h
                                                       int64_t table_pages, int64_t window, int64_t sinks) {
   Plan p;
   if (rldx_kv4_page_bytes(page_tokens, head_dim) < 0 || table_pages < 0 || table_pages > kMaxSlots / page_tokens ||
-      !plan_of(p, batch, q_heads, kv_heads, seq_q, table_pages * page_tokens, head_dim, window, sinks))
+      !plan_of(p, batch, q_heads, kv_heads, seq_q, table_pages * page_tokens, head_dim, window, sinks, true))
     return -1;
   return p.workspace(head_dim);
 }
@@ -1326,7 +1373,7 @@ extern "C" hipError_t rldx_kv4_attention_bf16(const void* q, const int64_t* q_st
   Plan p;
   if (!kv4_cache_ok(cache) || !common_ok(q, q_strides, o, o_strides, scale) ||
       !plan_of(p, batch, q_heads, cache->kv_heads, seq_q, cache->table_pages * cache->page_tokens, cache->head_dim,
-               window, sinks))
+               window, sinks, true))
     return hipErrorInvalidValue;
   if (batch == 0 || q_heads == 0 || seq_q == 0) return hipSuccess;
   if (!q || !o || !starts) return hipErrorInvalidValue;
