@@ -61,6 +61,7 @@ struct StreamArgs {
   int limit;              // readable keys: seq_k, or the slots of a row of the table
   int batch, sq, hq, hkv, group, window, sinks;
   int row_tiles, splits;
+  DivMagic d_group, d_hkv, d_row_tiles, d_splits;
   float scale_log2;
   float* part;  // [batch hkv row_tiles splits][rows per tile][D] O, then the same rows' {reference, sum}
 };
@@ -74,18 +75,29 @@ struct Span {
   int n;       // tiles in all
 };
 
+__device__ __forceinline__ int query_of(const StreamArgs& a, int row) {
+  return static_cast<int>(div_u32(static_cast<uint32_t>(row), a.d_group));
+}
+// id / d, and the rest of it into id
+__device__ __forceinline__ int split_off(int& id, int d, const DivMagic& by) {
+  const int q = static_cast<int>(div_u32(static_cast<uint32_t>(id), by));
+  const int rest = id - q * d;
+  id = q;
+  return rest;
+}
+
 template <bool kCache>
 __device__ __forceinline__ Span span_of(const StreamArgs& a, int b, int row0, int rows) {
   Span s;
   s.count = a.sq;
   if constexpr (kCache) {
-    s.start = min(max(a.starts[b], -kMaxSlots), kMaxSlots);
-    if (a.counts) s.count = min(s.count, a.counts[b]);
+    s.start = min(max(__builtin_amdgcn_readfirstlane(a.starts[b]), -kMaxSlots), kMaxSlots);
+    if (a.counts) s.count = min(s.count, __builtin_amdgcn_readfirstlane(a.counts[b]));
   } else {
     s.start = a.limit - a.sq;
   }
-  const int i0 = max(row0 / a.group, -min(s.start, 0));
-  const int i1 = min((row0 + rows - 1) / a.group, s.count - 1);
+  const int i0 = max(query_of(a, row0), -min(s.start, 0));
+  const int i1 = min(query_of(a, row0 + rows - 1), s.count - 1);
   s.p0 = s.start + i0;
   s.p1 = min(s.start + i1, a.limit - 1);  // (a query past the limit is NaN whatever it sees)
   if (i1 < i0 || s.p1 < s.p0) {
@@ -102,6 +114,10 @@ __device__ __forceinline__ Span span_of(const StreamArgs& a, int b, int row0, in
 
 // Splits that a row block of n tiles uses: none with less than one tile for each wave.
 __device__ __forceinline__ int splits_of(int splits, int n) { return max(1, min(splits, (n + kWaves - 1) / kWaves)); }
+// First tile of split x of use (n <= 2^25 tiles, x <= use <= 64)
+__device__ __forceinline__ int split_start(int n, int x, int use) {
+  return static_cast<int>(static_cast<uint32_t>(n) * static_cast<uint32_t>(x) / static_cast<uint32_t>(use));
+}
 
 // over the 4 lanes of a query (lanes l, l ^ 16, l ^ 32, l ^ 48): the swaps leave a lane's own value and its
 // partner's in the two registers
@@ -164,16 +180,6 @@ __device__ __forceinline__ uint32_t finite2(uint32_t w) {  // with zeros in the 
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
   return w;
 }
-// 1.0 where a half of the pair is of kind 0 .. 3 (+inf, -inf, NaN, NaN with a sign), else 0.
-__device__ __forceinline__ uint32_t marks2(uint32_t w, int kind) {
-  asm volatile("" : "+v"(w));
-  const uint32_t base = (kind & 1 ? 0xff80u : 0x7f80u) + (kind >> 1), more = kind >> 1 ? 0x7eu : 0u;
-  return ((w & 0xffffu) - base <= more ? 0x3f80u : 0u) | ((w >> 16) - base <= more ? 0x3f800000u : 0u);
-}
-__device__ __forceinline__ float mark_value(int kind) {
-  return kind == 0 ? __builtin_inff() : kind == 1 ? -__builtin_inff() : __builtin_nanf("");
-}
-
 // The keys 0 .. 31 of a tile that a query sees, a bit each: k0 <= p, and k0 > p - window or k0 < sinks.
 // s where bit c is set, else -inf
 __device__ __forceinline__ float seen_or_none(float s, uint32_t bits, int c) {
@@ -193,10 +199,9 @@ __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l
 
 template <int D, bool kCache>
 __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a) {
-  constexpr int KS = D / 32;          // MFMA steps over head_dim
-  constexpr int W = D / 16;           // dimensions of a lane's V columns, blocks of O^T
-  constexpr int OP = D + 4;           // pitch of O in LDS (floats)
-  constexpr int PF = kCache ? 2 : 1;  // tiles a wave has in flight
+  constexpr int KS = D / 32;  // MFMA steps over head_dim
+  constexpr int W = D / 16;   // dimensions of a lane's V columns, blocks of O^T
+  constexpr int OP = D + 4;   // pitch of O in LDS (floats)
   __shared__ __attribute__((aligned(16))) float sm_o[kWaves][kRowsBlock][OP];
   __shared__ float sm_ml[kWaves][kRowsBlock][2];
   const int lane = threadIdx.x & 63;
@@ -204,17 +209,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
   const int n16 = lane & 15, g = lane >> 4;
 
   // work item: (batch, kv head, split)
-  int id = static_cast<int>(blockIdx.x);
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int hk = id % a.hkv, b = id / a.hkv;
+  int b = static_cast<int>(blockIdx.x);
+  const int split = split_off(b, a.splits, a.d_splits), hk = split_off(b, a.hkv, a.d_hkv);
 
   const int rows = a.sq * a.group;  // <= kRowsBlock
   const Span sp = span_of<kCache>(a, b, 0, rows);
   const int use = splits_of(a.splits, sp.n);
   if (split >= use) return;
-  const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
-  const int t1 = static_cast<int>(static_cast<int64_t>(sp.n) * (split + 1) / use);
+  const int t0 = split_start(sp.n, split, use), t1 = split_start(sp.n, split + 1, use);
   const int mine = t1 - t0 > wave ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;  // tiles t0 + wave + 4 it
   auto tile_at = [&](int it) {
     const int t = t0 + wave + kWaves * it;
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
 
   // this lane's query: column n16 (the columns past the last row repeat it, and are not stored)
   const int row = min(n16, rows - 1);
-  const int qi = row / a.group, qh = hk * a.group + row - qi * a.group;
+  const int qi = query_of(a, row), qh = hk * a.group + row - qi * a.group;
   const int pos = qi < sp.count ? max(sp.start + qi, -1) : -1;  // slot, -1: sees nothing
   // every query sees something
   const bool all_rows = sp.p0 == sp.start && sp.p1 == sp.start + a.sq - 1;
@@ -312,11 +314,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
 #pragma unroll
   for (int j = 0; j < W; ++j) oacc[j] = floatx4{0, 0, 0, 0};
   float m_ref = -__builtin_inff(), l = 0.f;
+  bool odd_v = false;
+  auto whole = [&](int k0) {
+    return all_rows && k0 + kTile - 1 <= sp.p0 && (k0 > sp.p1 - a.window || k0 + kTile <= a.sinks);
+  };
 
   auto compute = [&](Raw<D, kCache>& raw, int it, int page) {
     const int k0 = tile_at(it) * kTile;
     // every query sees all 32 keys: no masks, and no key whose V may not be touched
-    bool full = page >= 0 && all_rows && k0 + kTile - 1 <= sp.p0 && (k0 > sp.p1 - a.window || k0 + kTile <= a.sinks);
+    bool full = page >= 0 && whole(k0);
     if constexpr (!kCache) {
       if (a.mask) {
         bool any = false, all = true;
@@ -351,8 +357,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
       }
     }
     // ---- visibility ----
-    bool odd_v = false;  // (wave-uniform) the tile's V holds something that is not finite
-    uint32_t vis = ~0u;
+    bool zero = false;  // (wave-uniform) V holds infinities or NaN that not every query sees
     if (!full) {
       uint32_t mbits = ~0u;  // bits 4 g .. + 3 and 16 + 4 g .. + 3: the others are not looked at
       if constexpr (!kCache) {
@@ -364,7 +369,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
             for (int r = 0; r < 4; ++r) mbits |= (raw.m[kt][r] != 0.f ? 1u : 0u) << (kt * 16 + g * 4 + r);
         }
       }
-      vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
+      const uint32_t vis = (visible_bits(k0, pos, a.window, a.sinks) & mbits) >> (4 * g);
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
           }
         }
       }
-      odd_v = __any(dirty || v.broken());
+      zero = __any(dirty || v.broken());
     }
     // ---- softmax ----
     float mt = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
@@ -448,28 +453,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
         vf[tp] = __builtin_amdgcn_perm(vr[2 * tp + 1][j / 2], vr[2 * tp][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
       return vf;
     };
-    if (odd_v) {
-      // Infinities and NaN of V go to the queries that see them, by products of what marks them with the visible
-      // keys, and leave zeros behind: a key that a query does not see weighs 0, and 0 times them would be NaN.
-      u32x4 seen;
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int c = 16 * (x >> 1) + 2 * (x & 1);
-        seen[x] = (vis & (1u << c) ? 0x3f80u : 0u) | (vis & (2u << c) ? 0x3f800000u : 0u);
-      }
-#pragma unroll 1
-      for (int kind = 0; kind < 4; ++kind)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          u32x4 vf = turn(j);
-#pragma unroll
-          for (int tp = 0; tp < 4; ++tp) vf[tp] = marks2(vf[tp], kind);
-          const floatx4 zero = {0, 0, 0, 0};
-          const floatx4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf),
-                                                                      __builtin_bit_cast(bf16x8, seen), zero, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) oacc[j][r] += hit[r] > 0.f ? mark_value(kind) : 0.f;
-        }
+    if (zero) {
+      // A key that a query does not see weighs 0, and 0 times an infinity or a NaN is a NaN: they go to the queries
+      // that see them behind the loop, and count as zeros here.
+      odd_v = true;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -481,19 +468,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
       oacc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, turn(j)), pf, oacc[j], 0, 0, 0);
   };
 
-  Raw<D, kCache> raw[PF];
-  int page[PF];
+  // (the next tile is on its way while this one is computed; two ahead took registers from a third workgroup on the CU:
+  // a token over 131072 cached slots 34.8 us, so 33.9)
+  Raw<D, kCache> next;
+  int next_page = -1;
+  if (mine > 0) load(next, 0, next_page);
+  for (int it = 0; it < mine; ++it) {
+    Raw<D, kCache> cur = next;
+    const int page = next_page;
+    if (it + 1 < mine) load(next, it + 1, next_page);
+    compute(cur, it, page);
+  }
+
+  if (__builtin_expect(odd_v, 0)) {  // this lane's dimensions: 4 W g .. + 4 W - 1, O^T element (j, r) the one at W r + j
+    for (int it = 0; it < mine; ++it) {
+      const int k0 = tile_at(it) * kTile;
+      uint32_t mbits = ~0u;
+      if constexpr (!kCache) {
+        if (a.mask) mbits = static_cast<uint32_t>(__ballot(a.mask[b * a.mask_sb + min(k0 + (lane & 31), a.limit - 1)] != 0.f));
+      }
+      if (mbits == 0 || (whole(k0) && mbits == ~0u)) continue;  // (whole tiles: the products have them)
+      const uint8_t* sc = nullptr;
+      if constexpr (kCache) {
+        const int page = __builtin_amdgcn_readfirstlane(a.table[b * a.table_sb + (k0 >> a.page_shift)]);
+        if (page < 0 || page >= a.num_pages) continue;
+        sc = a.cache + page * a.page_stride + hk * a.head_stride +
+             ((k0 & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D) + 33 * D + 4 * W * g / 32 * 32;
+      }
+      for (uint32_t vis = visible_bits(k0, pos, a.window, a.sinks) & mbits; vis; vis &= vis - 1) {
+        const int key = __builtin_ctz(vis);
+        if constexpr (kCache) {
+          if (sc[kv4::v_group(key) * 8 + kv4::v_unit(key)] >= 253)
 #pragma unroll
-  for (int u = 0; u < PF; ++u)
-    if (u < mine) load(raw[u], u, page[u]);
-  for (int it = 0; it < mine; it += PF) {
+            for (int j = 0; j < W; ++j) oacc[j] += __builtin_nanf("");
+        } else {
+          const uint16_t* const src = a.v + b * a.v_sb + hk * a.v_sh + static_cast<int64_t>(k0 + key) * a.v_ss + 4 * W * g;
 #pragma unroll
-    for (int u = 0; u < PF; ++u) {
-      if (it + u >= mine) break;
-      Raw<D, kCache> cur = raw[u];
-      const int pg = page[u];
-      if (it + u + PF < mine) load(raw[u], it + u + PF, page[u]);
-      compute(cur, it + u, pg);
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+              const uint16_t w = src[W * r + j];
+              if ((w & 0x7f80) == 0x7f80) oacc[j][r] += bf16_bits_to_f32(w);
+            }
+        }
+      }
     }
   }
 
@@ -535,7 +553,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
   }
   if (a.splits == 1) {
     const float inv = inverse_sum(lt);
-    const int i = mr / a.group, h = hk * a.group + mr - i * a.group;
+    const int i = query_of(a, mr), h = hk * a.group + mr - i * a.group;
     uint32_t out[W / 2];
 #pragma unroll
     for (int j = 0; j < W; j += 2) out[j / 2] = pack_bf16x2(acc[j] * inv, acc[j + 1] * inv);
@@ -644,19 +662,16 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
     const int per = total / 8, rem = total % 8, xcd = i % 8, k = i / 8;
     id = xcd < rem ? xcd * (per + 1) + k : rem * (per + 1) + (xcd - rem) * per + k;
   }
-  const int split = id % a.splits;
-  id /= a.splits;
-  const int rt = a.row_tiles - 1 - id % a.row_tiles;  // (the last rows first: they may have the longest spans)
-  id /= a.row_tiles;
-  const int hk = id % a.hkv, b = id / a.hkv;
+  const int split = split_off(id, a.splits, a.d_splits);
+  const int rt = a.row_tiles - 1 - split_off(id, a.row_tiles, a.d_row_tiles);  // (the last rows first: they may have the longest spans)
+  const int hk = split_off(id, a.hkv, a.d_hkv), b = id;
 
   const int rows = a.sq * a.group;
   const int row0 = rt * RB, rw0 = row0 + 32 * wq;
   const Span sp = span_of<kCache>(a, b, row0, min(RB, rows - row0));
   const int use = splits_of(a.splits, sp.n);
   if (split >= use) return;
-  const int t0 = static_cast<int>(static_cast<int64_t>(sp.n) * split / use);
-  const int n = static_cast<int>(static_cast<int64_t>(sp.n) * (split + 1) / use) - t0;
+  const int t0 = split_start(sp.n, split, use), n = split_start(sp.n, split + 1, use) - t0;
   auto tile_at = [&](int it) {
     const int t = t0 + min(it, n - 1);  // (past the end: the last one again)
     return t < sp.ns ? t : sp.w0 + (t - sp.ns);
@@ -664,9 +679,9 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
 
   // this lane's query, and the first and last slot of the wave's queries
   const int row = min(rw0 + l32, rows - 1);
-  const int qi = row / a.group, qh = hk * a.group + row - qi * a.group;
+  const int qi = query_of(a, row), qh = hk * a.group + row - qi * a.group;
   const int pos = qi < sp.count ? max(sp.start + qi, -1) : -1;
-  const int pw0 = sp.start + rw0 / a.group, pw1 = sp.start + (min(rw0 + 32, rows) - 1) / a.group;
+  const int pw0 = sp.start + query_of(a, rw0), pw1 = sp.start + query_of(a, min(rw0 + 32, rows) - 1);
   // (every query of the wave sees something)
   const bool all_rows = rw0 < rows && pw0 >= 0 && pw0 >= sp.p0 && pw1 <= sp.p1;
   bf16x8 qf[KCH];
@@ -1129,7 +1144,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
     const u32x4 w = *reinterpret_cast<const u32x4*>(st + r * OP + c);
     const int orow = rw0 + r;
     if (orow >= rows) continue;
-    const int i = orow / a.group, h = hk * a.group + orow - i * a.group;
+    const int i = query_of(a, orow), h = hk * a.group + orow - i * a.group;
     *reinterpret_cast<u32x4*>(a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + c) = w;
   }
 }
@@ -1201,7 +1216,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb
     }
   }
   const float inv = inverse_sum(l);
-  const int i = row / a.group, h = hk * a.group + row - i * a.group;
+  const int i = query_of(a, row), h = hk * a.group + row - i * a.group;
   uint16_t* const dst = a.o + b * a.o_sb + i * a.o_ss + h * a.o_sh + lane * E;
   if constexpr (E == 2)
     *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
@@ -1273,6 +1288,10 @@ void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* 
   a.sinks = static_cast<int>(std::min<int64_t>(sinks, kMaxSlots));
   a.row_tiles = p.row_tiles;
   a.splits = p.splits;
+  a.d_group = div_magic(static_cast<uint32_t>(a.group));
+  a.d_hkv = div_magic(static_cast<uint32_t>(a.hkv));
+  a.d_row_tiles = div_magic(static_cast<uint32_t>(a.row_tiles));
+  a.d_splits = div_magic(static_cast<uint32_t>(a.splits));
   a.scale_log2 = scale * kLog2e;
   a.part = static_cast<float*>(workspace);
 }

@@ -229,6 +229,27 @@ def test_append_special_values(dev, D):
         assert torch.equal(g, w) and torch.equal(torch.signbit(g), torch.signbit(w))
 
 
+def test_append_every_bf16_value(dev):
+    """All 65536 values, in blocks whose largest magnitude runs over mantissas and exponents, and in blocks of their
+    own, against the format in 64 bits, which the CPU tests hold the format's definition to."""
+    every = torch.arange(65536, dtype=torch.int32)
+    parts = [every[:, None].expand(-1, 32)]
+    for top in (0x3F80, 0x3FDF, 0x3FE0, 0x3FE1, 0x3FFF, 0x0001, 0x007F, 0x0080, 0x0100, 0x7F00, 0x7F60, 0x7F7F, 0x4123):
+        rows = torch.cat([every, every[: 2115 * 31 - 65536]]).view(2115, 31)
+        parts.append(torch.cat([torch.full((2115, 1), top, dtype=torch.int32), rows], 1))
+    x = torch.cat(parts)
+    x = torch.cat([x, x[: -x.shape[0] % 8]]).to(torch.int16).view(BF16).view(1, -1, 2, 128).to(dev)
+    S = x.shape[1]
+    c, table = cache_of(dev, 1, S, 2, 128, 256)
+    Fn.kv4_append(c, x, x.flip(1), table, ints(dev, 0))
+    rk, rv = Fn.kv4_read(c, table, ints(dev, 0), S, 128)
+    want = nearest(x)
+    for got, w in ((rk, want), (rv, want.flip(1))):
+        assert torch.equal(torch.isnan(got), torch.isnan(w))
+        g, w = torch.nan_to_num(got.double()), torch.nan_to_num(w)
+        assert torch.equal(g, w) and torch.equal(torch.signbit(g), torch.signbit(w))
+
+
 def test_append_and_read_skip_what_is_not_there(dev):
     """Slots below 0, past the table and of pages outside the cache are not written, and read as NaN."""
     c, table = cache_of(dev, 3, 128, 2, 128, 32)
