@@ -32,62 +32,66 @@ __device__ __forceinline__ uint8_t* tile_of(const Kv4Args& a, int b, int64_t slo
   return a.cache + page * a.page_stride + h * a.head_stride + (in / kv4::kTile) * kv4::tile_bytes(D);
 }
 
-// One thread per 8 dimensions of a row of K or V; the 4 threads of a block of 32 share its largest
-// magnitude.  Rows of a sequence are consecutive in the grid and the heads of a row adjacent, as the
-// rows lie in memory.  Bound by the stream: 2 x 2 D bytes of a row in, 2 (D/2 + D/32) out.
+// One workgroup per tile of the cache that the rows reach, one thread per 8 dimensions of a row of K and of V; the 4
+// threads of a block of 32 share its largest magnitude.  Bound by the stream: 2 x 2 D bytes of a row in, 2 (D/2 + D/32)
+// out.  4 x 8192 rows of 8 heads of 128, 170 MB: 37 us, 4.6 TB/s (a copy of that size reaches 4.9).  A thread per row
+// piece in the rows' own order (heads next to each other) took 49 us: a line of V codes holds a unit of each of 8 slots,
+// which then left through the caches of several XCDs, and every thread divided its way to its row.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4Args a) {
   constexpr int TPR = D / 8;  // threads per row
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int d0 = static_cast<int>(idx % TPR) * 8;
-  const int64_t row = idx / TPR;  // (b, i, h)
-  const int h = static_cast<int>(row % a.heads);
-  const int64_t bi = row / a.heads;
-  const int b = static_cast<int>(bi / a.seq), i = static_cast<int>(bi - static_cast<int64_t>(b) * a.seq);
-  if (b >= a.batch) return;  // whole rows: the threads of a block leave together
-  if (a.counts && i >= a.counts[b]) return;
-  const int64_t slot = static_cast<int64_t>(a.starts[b]) + i;
-  uint8_t* const t = tile_of(a, b, slot, h, D);
+  const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
+  const int64_t start = a.starts[b];
+  const int64_t slot0 = ((start >> 5) + blockIdx.x) * kv4::kTile;
+  const int n = a.counts ? min(a.seq, a.counts[b]) : a.seq;
+  uint8_t* const t = tile_of(a, b, slot0, h, D);
   if (!t) return;
-  const int s = static_cast<int>(slot) & (kv4::kTile - 1);
-  const u32x4 kx = *reinterpret_cast<const u32x4*>(a.k + b * a.k_sb + i * a.k_ss + h * a.k_sh + d0);
-  const u32x4 vx = *reinterpret_cast<const u32x4*>(a.v + b * a.v_sb + i * a.v_ss + h * a.v_sh + d0);
-  uint32_t codes[2];
-  uint32_t scale[2];
+  const int d0 = static_cast<int>(threadIdx.x) % TPR * 8;
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const u32x4 x = kv ? vx : kx;
-    uint32_t m = 0;
+  for (int s = static_cast<int>(threadIdx.x) / TPR; s < kv4::kTile; s += 256 / TPR) {
+    const int64_t i = slot0 + s - start;
+    if (i < 0 || i >= n) continue;  // whole rows: the threads of a block leave together
+    const u32x4 kx = *reinterpret_cast<const u32x4*>(a.k + b * a.k_sb + i * a.k_ss + h * a.k_sh + d0);
+    const u32x4 vx = *reinterpret_cast<const u32x4*>(a.v + b * a.v_sb + i * a.v_ss + h * a.v_sh + d0);
+    uint32_t codes[2];
+    uint32_t scale[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = x[j];
-      m = max(m, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+    for (int kv = 0; kv < 2; ++kv) {
+      const u32x4 x = kv ? vx : kx;
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = x[j];
+        m = max(m, max((w << 16) & 0x7fffffffu, w & 0x7fff0000u));
+      }
+      m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1)));
+      m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 2)));
+      const int e = kv4::block_exponent(m);
+      // (element_code of two values in one instruction: v_cvt_scalef32_pk_fp4_bf16 divides by the scale, rounds ties to
+      // the even code and cuts off at 6)
+      const float s2 = __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23);
+      const uint32_t w0 = x[0], w1 = x[1], w2 = x[2], w3 = x[3];
+      uint32_t c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w0), s2, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w1), s2, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w2), s2, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, w3), s2, 3);
+      codes[kv] = c;
+      scale[kv] = m >= 0x7f800000u ? kv4::kScaleNan : static_cast<uint32_t>(e + 127);
     }
-    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 1)));
-    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), 2)));
-    const int e = kv4::block_exponent(m);
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = x[j];
-      c |= kv4::element_code(bf16x2_lo(w), e) << (8 * j);
-      c |= kv4::element_code(bf16x2_hi(w), e) << (8 * j + 4);
+    *reinterpret_cast<uint32_t*>(t + s * (D / 2) + d0 / 2) = codes[0];
+    uint8_t* const vt = t + 16 * D;
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint32_t*>(vt + ((kv4::v_group(s) * 16 + d0 / 8) * 8 + kv4::v_unit(s)) * 4) = codes[1];
+    } else {
+      uint16_t* const u = reinterpret_cast<uint16_t*>(vt) + (kv4::v_group(s) * 16 + d0 / 4) * 8 + kv4::v_unit(s);
+      u[0] = static_cast<uint16_t>(codes[1]);
+      u[8] = static_cast<uint16_t>(codes[1] >> 16);
     }
-    codes[kv] = c;
-    scale[kv] = m >= 0x7f800000u ? kv4::kScaleNan : static_cast<uint32_t>(e + 127);
-  }
-  *reinterpret_cast<uint32_t*>(t + s * (D / 2) + d0 / 2) = codes[0];
-  uint8_t* const vt = t + 16 * D;
-  if constexpr (D == 128) {
-    *reinterpret_cast<uint32_t*>(vt + ((kv4::v_group(s) * 16 + d0 / 8) * 8 + kv4::v_unit(s)) * 4) = codes[1];
-  } else {
-    uint16_t* const u = reinterpret_cast<uint16_t*>(vt) + (kv4::v_group(s) * 16 + d0 / 4) * 8 + kv4::v_unit(s);
-    u[0] = static_cast<uint16_t>(codes[1]);
-    u[8] = static_cast<uint16_t>(codes[1] >> 16);
-  }
-  if (d0 % 32 == 0) {
-    t[32 * D + s * (D / 32) + d0 / 32] = static_cast<uint8_t>(scale[0]);
-    t[33 * D + (d0 / 32 * 4 + kv4::v_group(s)) * 8 + kv4::v_unit(s)] = static_cast<uint8_t>(scale[1]);
+    if (d0 % 32 == 0) {
+      t[32 * D + s * (D / 32) + d0 / 32] = static_cast<uint8_t>(scale[0]);
+      t[33 * D + (d0 / 32 * 4 + kv4::v_group(s)) * 8 + kv4::v_unit(s)] = static_cast<uint8_t>(scale[1]);
+    }
   }
 }
 
@@ -99,39 +103,40 @@ __device__ __forceinline__ u32x4 dequant8(uint32_t c, uint32_t scale_byte) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
-// The slots starts[b] .. + seq - 1 as bf16 rows; a slot that cannot be read gives NaN.
+// The slots starts[b] .. + seq - 1 as bf16 rows; a slot that cannot be read gives NaN.  Tiles and threads as above, for
+// the same reason: the 170 MB take 29 us, 33 in the rows' own order.
 template <int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4Args a) {
   constexpr int TPR = D / 8;
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int d0 = static_cast<int>(idx % TPR) * 8;
-  const int64_t row = idx / TPR;
-  const int h = static_cast<int>(row % a.heads);
-  const int64_t bi = row / a.heads;
-  const int b = static_cast<int>(bi / a.seq), i = static_cast<int>(bi - static_cast<int64_t>(b) * a.seq);
-  if (b >= a.batch) return;
-  const int64_t slot = static_cast<int64_t>(a.starts[b]) + i;
-  const uint8_t* const t = tile_of(a, b, slot, h, D);
-  u32x4 kx, vx;
-  if (t) {
-    const int s = static_cast<int>(slot) & (kv4::kTile - 1);
-    const uint8_t* const vt = t + 16 * D;
-    const uint32_t kc = *reinterpret_cast<const uint32_t*>(t + s * (D / 2) + d0 / 2);
-    uint32_t vc;
-    if constexpr (D == 128) {
-      vc = *reinterpret_cast<const uint32_t*>(vt + ((kv4::v_group(s) * 16 + d0 / 8) * 8 + kv4::v_unit(s)) * 4);
+  const int h = static_cast<int>(blockIdx.y), b = static_cast<int>(blockIdx.z);
+  const int64_t start = a.starts[b];
+  const int64_t slot0 = ((start >> 5) + blockIdx.x) * kv4::kTile;
+  const uint8_t* const t = tile_of(a, b, slot0, h, D);
+  const int d0 = static_cast<int>(threadIdx.x) % TPR * 8;
+#pragma unroll
+  for (int s = static_cast<int>(threadIdx.x) / TPR; s < kv4::kTile; s += 256 / TPR) {
+    const int64_t i = slot0 + s - start;
+    if (i < 0 || i >= a.seq) continue;
+    u32x4 kx, vx;
+    if (t) {
+      const uint8_t* const vt = t + 16 * D;
+      const uint32_t kc = *reinterpret_cast<const uint32_t*>(t + s * (D / 2) + d0 / 2);
+      uint32_t vc;
+      if constexpr (D == 128) {
+        vc = *reinterpret_cast<const uint32_t*>(vt + ((kv4::v_group(s) * 16 + d0 / 8) * 8 + kv4::v_unit(s)) * 4);
+      } else {
+        const uint16_t* const u =
+            reinterpret_cast<const uint16_t*>(vt) + (kv4::v_group(s) * 16 + d0 / 4) * 8 + kv4::v_unit(s);
+        vc = u[0] | static_cast<uint32_t>(u[8]) << 16;
+      }
+      kx = dequant8(kc, t[32 * D + s * (D / 32) + d0 / 32]);
+      vx = dequant8(vc, t[33 * D + (d0 / 32 * 4 + kv4::v_group(s)) * 8 + kv4::v_unit(s)]);
     } else {
-      const uint16_t* const u =
-          reinterpret_cast<const uint16_t*>(vt) + (kv4::v_group(s) * 16 + d0 / 4) * 8 + kv4::v_unit(s);
-      vc = u[0] | static_cast<uint32_t>(u[8]) << 16;
+      kx = vx = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
     }
-    kx = dequant8(kc, t[32 * D + s * (D / 32) + d0 / 32]);
-    vx = dequant8(vc, t[33 * D + (d0 / 32 * 4 + kv4::v_group(s)) * 8 + kv4::v_unit(s)]);
-  } else {
-    kx = vx = u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    *reinterpret_cast<u32x4*>(a.k + b * a.k_sb + i * a.k_ss + h * a.k_sh + d0) = kx;
+    *reinterpret_cast<u32x4*>(a.v + b * a.v_sb + i * a.v_ss + h * a.v_sh + d0) = vx;
   }
-  *reinterpret_cast<u32x4*>(a.k + b * a.k_sb + i * a.k_ss + h * a.k_sh + d0) = kx;
-  *reinterpret_cast<u32x4*>(a.v + b * a.v_sb + i * a.v_ss + h * a.v_sh + d0) = vx;
 }
 
 bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -147,9 +152,7 @@ hipError_t kv4_args(Kv4Args& a, const rldx_kv4_cache_t* c, const void* k, const 
   if (!k || !v || !starts || !a16(k) || !a16(v)) return hipErrorInvalidValue;
   for (int i = 0; i < 3; ++i)
     if (ks[i] % 8 || vs[i] % 8) return hipErrorInvalidValue;
-  if (seq > (int64_t{1} << 30) || batch > 65535 ||
-      (batch * seq * c->kv_heads * (c->head_dim / 8) + 255) / 256 > (int64_t{1} << 31) - 1)
-    return hipErrorInvalidValue;
+  if (seq > (int64_t{1} << 28) || batch > 65535) return hipErrorInvalidValue;
   a.cache = static_cast<uint8_t*>(c->data);
   a.page_stride = c->page_stride;
   a.head_stride = c->head_stride;
@@ -171,8 +174,10 @@ hipError_t kv4_args(Kv4Args& a, const rldx_kv4_cache_t* c, const void* k, const 
   return hipSuccess;
 }
 
-unsigned grid_of(const Kv4Args& a, int64_t D) {
-  return static_cast<unsigned>((static_cast<int64_t>(a.batch) * a.seq * a.heads * (D / 8) + 255) / 256);
+// tiles that seq rows may reach, from wherever they start
+dim3 tile_grid(const Kv4Args& a) {
+  return dim3(static_cast<unsigned>((a.seq + 2 * kv4::kTile - 2) / kv4::kTile), static_cast<unsigned>(a.heads),
+              static_cast<unsigned>(a.batch));
 }
 
 }  // namespace
@@ -225,9 +230,9 @@ extern "C" hipError_t rldx_kv4_append_bf16(const rldx_kv4_cache_t* cache, const 
   const hipError_t e = kv4_args(a, cache, k, k_strides, v, v_strides, starts, counts, batch, seq, &work);
   if (e != hipSuccess || !work) return e;
   if (cache->head_dim == 128)
-    hipLaunchKernelGGL(kv4_append_kernel<128>, dim3(grid_of(a, 128)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_append_kernel<128>, tile_grid(a), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL(kv4_append_kernel<64>, dim3(grid_of(a, 64)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_append_kernel<64>, tile_grid(a), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -239,8 +244,8 @@ extern "C" hipError_t rldx_kv4_read_bf16(const rldx_kv4_cache_t* cache, const in
   const hipError_t e = kv4_args(a, cache, k, k_strides, v, v_strides, starts, nullptr, batch, seq, &work);
   if (e != hipSuccess || !work) return e;
   if (cache->head_dim == 128)
-    hipLaunchKernelGGL(kv4_read_kernel<128>, dim3(grid_of(a, 128)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_read_kernel<128>, tile_grid(a), dim3(256), 0, stream, a);
   else
-    hipLaunchKernelGGL(kv4_read_kernel<64>, dim3(grid_of(a, 64)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_read_kernel<64>, tile_grid(a), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
