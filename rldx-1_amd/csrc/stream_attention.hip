@@ -12,8 +12,8 @@
 // and P^T goes from the S^T accumulators to the B operand without leaving its lane: lane group g
 // holds keys 4 g .. 4 g + 3 of both blocks, and the V^T operand takes its 32 keys in that order.
 // V rows are turned by v_perm on pairs of rows that the lane itself has loaded (8 keys by head_dim / 16
-// dimensions a lane), so nothing goes through LDS but the merge of the workgroup's 4 waves, which
-// walk tiles w, w + 4, ...  Where the rows leave most CUs idle, `splits` workgroups share
+// dimensions a lane), so nothing goes through LDS but the merge of the workgroup's 4 or 8 waves, which
+// walk tiles w, w + 4 (8), ...  Where the rows leave most CUs idle, `splits` workgroups share
 // the tiles of a row block and merge_kernel adds up their partial states (fp32, as the softmax
 // reference, the sum and the unnormalised O).
 #include <algorithm>
@@ -197,13 +197,13 @@ __device__ __forceinline__ float rescale(float m, float n) { return __builtin_am
 // 1 / sum of a softmax: a query that has seen nothing has O = 0; a NaN stays.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : l == 0.f ? 1.f : l; }
 
-template <int D, bool kCache>
-__global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a) {
+template <int D, bool kCache, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void rows_attn_kernel(StreamArgs a) {
   constexpr int KS = D / 32;  // MFMA steps over head_dim
   constexpr int W = D / 16;   // dimensions of a lane's V columns, blocks of O^T
   constexpr int OP = D + 4;   // pitch of O in LDS (floats)
-  __shared__ __attribute__((aligned(16))) float sm_o[kWaves][kRowsBlock][OP];
-  __shared__ float sm_ml[kWaves][kRowsBlock][2];
+  __shared__ __attribute__((aligned(16))) float sm_o[NW][kRowsBlock][OP];
+  __shared__ float sm_ml[NW][kRowsBlock][2];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int n16 = lane & 15, g = lane >> 4;
@@ -217,9 +217,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
   const int use = splits_of(a.splits, sp.n);
   if (split >= use) return;
   const int t0 = split_start(sp.n, split, use), t1 = split_start(sp.n, split + 1, use);
-  const int mine = t1 - t0 > wave ? (t1 - t0 - wave + kWaves - 1) / kWaves : 0;  // tiles t0 + wave + 4 it
+  const int mine = t1 - t0 > wave ? (t1 - t0 - wave + NW - 1) / NW : 0;  // tiles t0 + wave + NW it
   auto tile_at = [&](int it) {
-    const int t = t0 + wave + kWaves * it;
+    const int t = t0 + wave + NW * it;
     return t < sp.ns ? t : sp.w0 + (t - sp.ns);
   };
 
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
     }
   }
 
-  // ---- merge the 4 waves ----
+  // ---- merge the waves ----
   const float lsum = quad_sum(l);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -533,12 +533,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
   __syncthreads();
   const int tid = static_cast<int>(threadIdx.x);
   const int mr = tid >> 4, md = (tid & 15) * W;  // the row and the first of W dimensions that this thread finishes
-  if (mr >= rows) return;
-  float m = -__builtin_inff(), lt = 0.f, w[kWaves];
+  if (mr >= rows) return;  // (and all threads past the first 256)
+  float m = -__builtin_inff(), lt = 0.f, w[NW];
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
+  for (int i = 0; i < NW; ++i) m = fmaxf(m, sm_ml[i][mr][0]);
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
+  for (int i = 0; i < NW; ++i) {
     w[i] = rescale(sm_ml[i][mr][0], m);
     lt = __builtin_fmaf(sm_ml[i][mr][1], w[i], lt);
   }
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void rows_attn_kernel(StreamArgs a)
   for (int j = 0; j < W; j += 4) {
     floatx4 x = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) x += *reinterpret_cast<const floatx4*>(&sm_o[i][mr][md + j]) * w[i];
+    for (int i = 0; i < NW; ++i) x += *reinterpret_cast<const floatx4*>(&sm_o[i][mr][md + j]) * w[i];
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[j + e] = x[e];
   }
@@ -1231,6 +1231,7 @@ bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How a call is cut up; depends on sizes alone.
 struct Plan {
+  int waves;                  // of a rows_attn_kernel workgroup: 4, or 8 for a row block that is not split
   int rb, row_tiles, splits;  // rows of a workgroup: 16 (rows_attn_kernel), 32, 64 or 128 (tile_attn_kernel)
   int64_t items;  // row blocks times splits
   int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * rb * (head_dim + 2) * 4 : 0; }
@@ -1264,6 +1265,16 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
                                  (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
   const int64_t want = std::max<int64_t>(1, (p.rb == kRowsBlock ? 2 : 1) * cus / blocks);
   p.splits = static_cast<int>(std::min<int64_t>({kMaxSplits, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
+  // Sharing a row block out means a second launch, about 3 us.  Where 8 waves walk the tiles in (nearly) as few steps as
+  // 4 waves of each split do, one workgroup of 8 takes the row block whole.  A step takes a workgroup 0.5 us (codes,
+  // head_dim 64), 0.9 (codes, or rows of 64) or 1.7 (rows of 128, 128 KB).  Token of 32/8 heads of 128, shared out ->
+  // whole: 250 slots 7.4 -> 4.9, 1500 slots 7.7 (10.1 whole), 32 sequences of 1500 slots 16.1 -> 12.7; bf16 rows: 250 keys
+  // 7.9 -> 6.1, 500 keys 7.9 (8.6 whole), 32 sequences of 1000 keys 29.3 -> 25.9.
+  p.waves = 4;
+  if (p.rb == kRowsBlock && p.splits > 1) {
+    const int64_t more = (tiles + 7) / 8 - (tiles + 4 * p.splits - 1) / (4 * p.splits);
+    if (more <= (!cache && head_dim == 128 ? 0 : 2)) p.waves = 8, p.splits = 1;
+  }
   p.items = blocks * p.splits;
   return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
 }
@@ -1308,9 +1319,12 @@ void launch_tiles(const StreamArgs& a, dim3 grid, hipStream_t stream) {
 
 template <int D, bool kCache>
 hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.items)), block(64 * kWaves);
+  const dim3 grid(static_cast<unsigned>(p.items));
   if (p.rb == kRowsBlock)
-    hipLaunchKernelGGL((rows_attn_kernel<D, kCache>), grid, block, 0, stream, a);
+    if (p.waves == 8)
+      hipLaunchKernelGGL((rows_attn_kernel<D, kCache, 8>), grid, dim3(64 * 8), 0, stream, a);
+    else
+      hipLaunchKernelGGL((rows_attn_kernel<D, kCache, 4>), grid, dim3(64 * 4), 0, stream, a);
   else if (p.rb == 32)
     launch_tiles<D, 4, kCache>(a, grid, stream);
   else if (p.rb == 64)
@@ -1321,8 +1335,8 @@ hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
   if (e != hipSuccess || p.splits == 1) return e;
   const int per = p.splits <= kMaxSplits / kWaves ? 1 : kWaves;  // waves to a row
   const int64_t out_rows = static_cast<int64_t>(a.batch) * a.hq * a.sq;
-  hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>((out_rows * per + kWaves - 1) / kWaves)), block, 0,
-                     stream, a, p.rb, per);
+  hipLaunchKernelGGL((merge_kernel<D, kCache>), dim3(static_cast<unsigned>((out_rows * per + kWaves - 1) / kWaves)),
+                     dim3(64 * kWaves), 0, stream, a, p.rb, per);
   return hipGetLastError();
 }
 
