@@ -633,9 +633,9 @@ __device__ __forceinline__ void read_v(u32x2 (&v0)[2][2], u32x2 (&v1)[2][2], uin
       : "memory");
 }
 
-template <int D, int NG, bool kCache, bool kMask>
-__global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && (kCache || kMask)) ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
-  constexpr int NQ = kWaves / NG, RB = 32 * NQ;
+template <int D, int NG, bool kCache, bool kMask, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D == 128 && (kCache || kMask)) ? 2 : 3) void tile_attn_kernel(StreamArgs a) {
+  constexpr int NQ = NW / NG, RB = 32 * NQ;
   constexpr int KCH = D / 16;      // MFMA steps over head_dim
   constexpr int DBLK = D / 32;     // 32-dimension blocks of O^T
   constexpr int PCS = D / 8;       // 16-byte pieces of a row
@@ -645,14 +645,17 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
   constexpr int TILEB = 2 * 32 * ROWB;   // K and V of a tile in LDS; a ring slot holds NG tiles, a step's
   constexpr int NS = kCache || NG > 1 ? 2 : 3;  // ring slots
   constexpr int OP = D + 8;              // pitch of O rows staged in LDS
-  constexpr int RING = NS * NG * TILEB, STAGE = kWaves * 32 * OP * 2;
+  constexpr int RING = NS * NG * TILEB, STAGE = NW * 32 * OP * 2;
+  constexpr int FT = 4 * NG / NW;        // cache: tiles of a step that 4 waves turn into values
   static_assert(NG == 1 || NG == 2 || NG == 4, "key groups");
-  constexpr int EXCH = NG > 1 ? kWaves * (DBLK * 4 + 1) * 1024 : 0;  // states that the key groups exchange
+  static_assert(NW == kWaves || (kCache && NW == 8 && NG > 1), "waves");
+  constexpr int EXCH = NG > 1 ? NW * (DBLK * 4 + 1) * 1024 : 0;  // states that the key groups exchange
   constexpr int LDS = RING > STAGE ? (RING > EXCH ? RING : EXCH) : (STAGE > EXCH ? STAGE : EXCH);
   __shared__ __attribute__((aligned(1024))) uint8_t ring[LDS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l32 = lane & 31, g = lane >> 5;
+  const int fg = wave / 4;
   const int wq = wave % NQ, kg = wave / NQ;  // the wave's block of 32 rows, and its share of the tiles
 
   // work item: (batch, kv head, row tile, split), neighbours on one XCD (workgroup i runs on XCD i % 8)
@@ -767,14 +770,14 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
     scales = 0;
     if (page < 0) return;
     const uint8_t* const t = tile_ptr(page, it);
-    const uint8_t* const src = t + (wave < 2 ? 0 : 16 * D) + ct * (D / 8);
+    const uint8_t* const src = t + ((wave & 3) < 2 ? 0 : 16 * D) + ct * (D / 8);
     if constexpr (D == 128) {
       codes = *reinterpret_cast<const u32x4*>(src);
     } else {
       const u32x2 x = *reinterpret_cast<const u32x2*>(src);
       codes = u32x4{x[0], x[1], 0, 0};
     }
-    if (wave < 2) {
+    if ((wave & 3) < 2) {
       scales = t[32 * D + (ct >> 2) * (D / 32) + (D == 128 ? ct & 3 : (ct & 3) >> 1)];
     } else {  // the scales of 4 slots
       const int lb = ct >> 1;
@@ -783,7 +786,7 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
   };
   auto store = [&](int off, u32x4 codes, uint32_t scales) {
     uint8_t* const ks = ring + off;
-    if (wave < 2) {
+    if ((wave & 3) < 2) {
       const int r = ct >> 2;
       const float sc = __builtin_bit_cast(float, scales << 23);
 #pragma unroll
@@ -964,22 +967,22 @@ __global__ __launch_bounds__(64 * kWaves, NG == 4 ? 1 : NG == 2 || (D == 128 && 
     const int steps = (n + NG - 1) / NG;
     if constexpr (kCache) {
       load_ids(0);
-      u32x4 codes[NG];
-      uint32_t scales[NG];
+      u32x4 codes[FT];
+      uint32_t scales[FT];
       int own = -1, own_next = -1;  // the page of this wave's tile
       auto fetch_step = [&](int st) {
         int mine = -1;
 #pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          const int page = st * NG + x < n ? page_of(st * NG + x) : -1;
-          fetch(page, st * NG + x, codes[x], scales[x]);
-          mine = x == kg ? page : mine;
+        for (int x = 0; x < FT; ++x) {
+          const int t = fg * FT + x, page = st * NG + t < n ? page_of(st * NG + t) : -1;
+          fetch(page, st * NG + t, codes[x], scales[x]);
+          mine = t == kg ? page : mine;
         }
         return mine;
       };
       auto store_step = [&](int slot) {
 #pragma unroll
-        for (int x = 0; x < NG; ++x) store((slot * NG + x) * TILEB, codes[x], scales[x]);
+        for (int x = 0; x < FT; ++x) store((slot * NG + fg * FT + x) * TILEB, codes[x], scales[x]);
       };
       own = fetch_step(0);
       store_step(0);
@@ -1231,7 +1234,7 @@ bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How a call is cut up; depends on sizes alone.
 struct Plan {
-  int waves;                  // of a rows_attn_kernel workgroup: 4, or 8 for a row block that is not split
+  int waves;                  // of a workgroup: 4 or 8
   int rb, row_tiles, splits;  // rows of a workgroup: 16 (rows_attn_kernel), 32, 64 or 128 (tile_attn_kernel)
   int64_t items;  // row blocks times splits
   int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * rb * (head_dim + 2) * 4 : 0; }
@@ -1246,31 +1249,49 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
   const int64_t group = q_heads / kv_heads, rows = seq_q * group;
   if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
   const int64_t heads = std::max<int64_t>(1, batch * kv_heads);
-  const auto row_tiles = [&](int64_t rb) { return (rows + rb - 1) / rb; };
-  // The smallest row blocks whose workgroups run all at once (per CU, by LDS and registers: 1 and 2 of 32 and 64 rows for
-  // head_dim 128, 2 and 4 for 64), else 128 rows.  Over the cache every block turns the codes into values again,
-  // so it takes 128 rows and splits the keys from 65 rows on.
+  // workgroups of 32 (bf16 rows; twice as many of 64) or 128 rows (codes, 8 waves) that a CU's LDS holds
   const int64_t cus = 256, per_cu = head_dim == 128 ? 1 : 2;
-  if (rows <= kRowsBlock)
+  const auto row_tiles = [&](int64_t rb) { return std::max<int64_t>(1, (rows + rb - 1) / rb); };
+  // tiles of the longest block of rb rows
+  const auto tiles_of = [&](int64_t rb) {
+    const int64_t span = std::min(limit, std::min(window, limit) + rb / std::max<int64_t>(1, group) + 1);
+    return std::min((limit + kTile - 1) / kTile,
+                    (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
+  };
+  const auto splits_for = [&](int64_t blocks, int64_t tiles, int64_t workgroups) {
+    return std::min<int64_t>({kMaxSplits, std::max<int64_t>(1, workgroups / blocks), std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)});
+  };
+  // steps that a CU takes, one after the other, over blocks of rb rows and `per` tiles a step
+  const auto steps_of = [&](int64_t rb, int64_t per) {
+    const int64_t blocks = heads * row_tiles(rb), tiles = tiles_of(rb), splits = splits_for(blocks, tiles, cus);
+    return ((tiles + splits - 1) / splits + per - 1) / per * ((blocks * splits + cus - 1) / cus);
+  };
+  p.waves = 4;
+  if (rows <= kRowsBlock) {
     p.rb = kRowsBlock;
-  else if (cache)
-    p.rb = rows <= 64 ? 32 : 128;
-  else
+  } else if (cache) {
+    // Every row block turns the codes into values again, 32 rows 4 times as often as 128, but the fewer rows, the more
+    // keys a step takes (4 tiles, 2 of 128 rows) and the fewer partial states leave the chip.  A step takes 2 us (32 rows,
+    // 4 waves; 64 rows, 8 waves), 1.3 (128 rows, 8 waves).  us for 32 / 64 / 128 rows, head_dim 128: 49 tokens of 28/4
+    // heads over 300 slots 12.3 / 14.1 / 15.1, over 6000 32.6 / 24.1 / 27.3, 2 sequences of them 58.7 / 34.7 / 32.3;
+    // 169 tokens over 500 slots 13.5 / 19.6 / 20.9, over 2000 36.5 / 26.5 / 29.0, over 20000 375 / 115 / 86.
+    p.rb = steps_of(32, 4) <= 4 ? 32 : steps_of(64, 4) <= 8 ? 64 : 128;
+    // Blocks of 128 rows that do not run at once: 4 waves, a tile a step (4096 tokens of 32/8 heads over 8192 slots 471
+    // us, 516 with 8 waves; 1024 tokens, which do, 246 and 172).
+    if (p.rb == 64 || (p.rb == 128 && heads * row_tiles(128) <= per_cu * cus)) p.waves = 8;
+  } else {
+    // The smallest row blocks whose workgroups run all at once, else 128 rows.  us for 32 / 64 / 128 rows, window: 169
+    // queries of 28/4 heads of 128 17 / 25 / 29, 640 of them 29 / 19 / 23, 8192 of 32/8 heads 443 / 223 / 172.
     p.rb = heads * row_tiles(32) <= per_cu * cus ? 32 : heads * row_tiles(64) <= 2 * per_cu * cus ? 64 : 128;
-  p.row_tiles = static_cast<int>(rows == 0 ? 1 : row_tiles(p.rb));
-  const int64_t blocks = heads * p.row_tiles;
-  // tiles of the longest row block
-  const int64_t span = std::min(limit, std::min(window, limit) + p.rb / std::max<int64_t>(1, group) + 1);
-  const int64_t tiles = std::min((limit + kTile - 1) / kTile,
-                                 (std::min(sinks, limit) + kTile - 1) / kTile + (span + kTile - 1) / kTile + 1);
-  const int64_t want = std::max<int64_t>(1, (p.rb == kRowsBlock ? 2 : 1) * cus / blocks);
-  p.splits = static_cast<int>(std::min<int64_t>({kMaxSplits, want, std::max<int64_t>(1, (tiles + kWaves - 1) / kWaves)}));
+  }
+  p.row_tiles = static_cast<int>(row_tiles(p.rb));
+  const int64_t blocks = heads * p.row_tiles, tiles = tiles_of(p.rb);
+  p.splits = static_cast<int>(splits_for(blocks, tiles, (p.rb == kRowsBlock ? 2 : 1) * cus));
   // Sharing a row block out means a second launch, about 3 us.  Where 8 waves walk the tiles in (nearly) as few steps as
   // 4 waves of each split do, one workgroup of 8 takes the row block whole.  A step takes a workgroup 0.5 us (codes,
   // head_dim 64), 0.9 (codes, or rows of 64) or 1.7 (rows of 128, 128 KB).  Token of 32/8 heads of 128, shared out ->
   // whole: 250 slots 7.4 -> 4.9, 1500 slots 7.7 (10.1 whole), 32 sequences of 1500 slots 16.1 -> 12.7; bf16 rows: 250 keys
   // 7.9 -> 6.1, 500 keys 7.9 (8.6 whole), 32 sequences of 1000 keys 29.3 -> 25.9.
-  p.waves = 4;
   if (p.rb == kRowsBlock && p.splits > 1) {
     const int64_t more = (tiles + 7) / 8 - (tiles + 4 * p.splits - 1) / (4 * p.splits);
     if (more <= (!cache && head_dim == 128 ? 0 : 2)) p.waves = 8, p.splits = 1;
@@ -1307,30 +1328,37 @@ void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* 
   a.part = static_cast<float*>(workspace);
 }
 
-template <int D, int NG, bool kCache>
+template <int D, int NG, bool kCache, int NW>
 void launch_tiles(const StreamArgs& a, dim3 grid, hipStream_t stream) {
   if constexpr (kCache)
-    hipLaunchKernelGGL((tile_attn_kernel<D, NG, true, false>), grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, true, false, NW>), grid, dim3(64 * NW), 0, stream, a);
   else if (a.mask)
-    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, true>), grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, true, NW>), grid, dim3(64 * NW), 0, stream, a);
   else
-    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, false>), grid, dim3(64 * kWaves), 0, stream, a);
+    hipLaunchKernelGGL((tile_attn_kernel<D, NG, false, false, NW>), grid, dim3(64 * NW), 0, stream, a);
 }
 
 template <int D, bool kCache>
 hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
   const dim3 grid(static_cast<unsigned>(p.items));
-  if (p.rb == kRowsBlock)
+  if (p.rb == kRowsBlock) {
     if (p.waves == 8)
       hipLaunchKernelGGL((rows_attn_kernel<D, kCache, 8>), grid, dim3(64 * 8), 0, stream, a);
     else
       hipLaunchKernelGGL((rows_attn_kernel<D, kCache, 4>), grid, dim3(64 * 4), 0, stream, a);
-  else if (p.rb == 32)
-    launch_tiles<D, 4, kCache>(a, grid, stream);
-  else if (p.rb == 64)
-    launch_tiles<D, 2, kCache>(a, grid, stream);
-  else
-    launch_tiles<D, 1, kCache>(a, grid, stream);
+  } else if (p.rb == 32) {
+    launch_tiles<D, 4, kCache, 4>(a, grid, stream);
+  } else if (p.rb == 64) {
+    if constexpr (kCache)
+      launch_tiles<D, 4, true, 8>(a, grid, stream);
+    else
+      launch_tiles<D, 2, false, 4>(a, grid, stream);
+  } else {
+    bool taken = false;
+    if constexpr (kCache)
+      if ((taken = p.waves == 8)) launch_tiles<D, 2, true, 8>(a, grid, stream);
+    if (!taken) launch_tiles<D, 1, kCache, 4>(a, grid, stream);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
   const int per = p.splits <= kMaxSplits / kWaves ? 1 : kWaves;  // waves to a row

@@ -369,6 +369,34 @@ def test_kv4_attention_nan_blocks(dev, D, Sq):
             check(Fn.kv4_attention(q, c, table, st, None, window, sinks), ref, bound, f"{which} {window} {sinks}")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", [  # batch, Sq, Hq, Hkv, slots, starts: one or two of each cut of the work
+    (2, 1, 32, 8, 250, (249, 100)), (16, 1, 24, 8, 1300, tuple(range(1299, 3, -81))), (1, 49, 28, 4, 6000, (5940,)),
+    (2, 49, 28, 4, 6000, (5951, 333)), (1, 70, 32, 8, 9000, (8900,)), (8, 300, 24, 24, 331, (31, 0, 30, 17, 1, 12, 29, 5))],
+    ids=str)
+def test_kv4_attention_long_chunks(dev, case, D):
+    """Chunks over long caches with NaN blocks in K and V, hidden from some queries by the order and the window, rows
+    past a sequence's count and a page that is missing."""
+    B, Sq, Hq, Hkv, slots, starts = case
+    k, v = rnd(dev, B, slots, Hkv, D, seed=1), rnd(dev, B, slots, Hkv, D, seed=2)
+    for b, st in enumerate(starts):
+        v[b, st + Sq - 1, Hkv - 1, D - 1] = v[b, max(st - 4, 0), 0, 3] = float("nan")
+        v[b, st + Sq // 2, b % Hkv, 40] = k[b, st + Sq - 1, 1, 0] = float("inf")
+        v[b, st // 3, 2, 0] = k[b, st // 2, 3, 9] = -float("inf")
+    c, table = cache_of(dev, B, slots, Hkv, D, 64)
+    Fn.kv4_append(c, k, v, table, ints(dev, *[0] * B))
+    q, st = rnd(dev, B, Sq, Hq, D, seed=3), ints(dev, *starts)
+    counts = ints(dev, *[Sq - (b % 3 == 1) for b in range(B)])
+    for window, sinks in ((None, 0), (70, 33)):
+        check(Fn.kv4_attention(q, c, table, st, counts, window, sinks),
+              *kv4_ref(q, c, table, st, counts, window, sinks), f"{window} {sinks}")
+    if starts[0] >= 250:
+        want = Fn.kv4_attention(q, c, table, st, counts, 70, 33)
+        table[0, 1] = -1
+        assert torch.equal(torch.nan_to_num(Fn.kv4_attention(q, c, table, st, counts, 70, 33)), torch.nan_to_num(want))
+        assert torch.isnan(Fn.kv4_attention(q, c, table, st, counts)[0, 0]).all()
+
+
 def test_kv4_offsets_past_32_bits(dev):
     """Pages more than 2^32 bytes behind the first one."""
     H, D, page = 8, 128, 64
