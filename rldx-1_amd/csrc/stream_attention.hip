@@ -61,7 +61,7 @@ struct StreamArgs {
   int limit;              // readable keys: seq_k, or the slots of a row of the table
   int batch, sq, hq, hkv, group, window, sinks;
   int row_tiles, splits;
-  DivMagic d_group, d_hkv, d_row_tiles, d_splits;
+  DivMagic d_group, d_hkv, d_row_tiles, d_splits, d_items;
   float scale_log2;
   float* part;  // [batch hkv row_tiles splits][rows per tile][D] O, then the same rows' {reference, sum}
 };
@@ -658,12 +658,21 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   const int fg = wave / 4;
   const int wq = wave % NQ, kg = wave / NQ;  // the wave's block of 32 rows, and its share of the tiles
 
-  // work item: (batch, kv head, row tile, split), neighbours on one XCD (workgroup i runs on XCD i % 8)
+  // Work item: (batch, kv head, row tile, split).  Workgroup i runs on XCD i % 8: the items of a pair (batch, kv head),
+  // which read the same keys, stay on one XCD, and the pairs go round the XCDs (sequences of a batch may differ in length:
+  // 8 padded ones of 777 tokens and 24 heads of 64 took 31.8 us with a sequence to an XCD, 29.4 so); the last pairs,
+  // fewer than 8, are cut into 8 runs of items.
   int id;
   {
-    const int total = static_cast<int>(gridDim.x), i = static_cast<int>(blockIdx.x);
-    const int per = total / 8, rem = total % 8, xcd = i % 8, k = i / 8;
-    id = xcd < rem ? xcd * (per + 1) + k : rem * (per + 1) + (xcd - rem) * per + k;
+    const int xcd = static_cast<int>(blockIdx.x % 8), k = static_cast<int>(blockIdx.x / 8);
+    const int items = a.row_tiles * a.splits, pairs = a.batch * a.hkv, round = pairs / 8 * items;
+    if (k < round) {
+      const int turn = static_cast<int>(div_u32(static_cast<uint32_t>(k), a.d_items));
+      id = k + (turn * 7 + xcd) * items;  // pair 8 turn + xcd, its item k - turn items
+    } else {
+      const int left = pairs % 8 * items, per = left / 8, more = left % 8;
+      id = round * 8 + (k - round) + xcd * per + min(xcd, more);
+    }
   }
   const int split = split_off(id, a.splits, a.d_splits);
   const int rt = a.row_tiles - 1 - split_off(id, a.row_tiles, a.d_row_tiles);  // (the last rows first: they may have the longest spans)
@@ -1324,6 +1333,7 @@ void fill(StreamArgs& a, const Plan& p, const void* q, const int64_t* qs, void* 
   a.d_hkv = div_magic(static_cast<uint32_t>(a.hkv));
   a.d_row_tiles = div_magic(static_cast<uint32_t>(a.row_tiles));
   a.d_splits = div_magic(static_cast<uint32_t>(a.splits));
+  a.d_items = div_magic(static_cast<uint32_t>(a.row_tiles) * static_cast<uint32_t>(a.splits));
   a.scale_log2 = scale * kLog2e;
   a.part = static_cast<float*>(workspace);
 }

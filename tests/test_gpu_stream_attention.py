@@ -109,6 +109,19 @@ def test_window_attention_key_mask(dev, sq, sk, D, Hq, Hkv):
     assert torch.equal(Fn.window_attention(q, k, v, 50, 3, big), o)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sq,window,sinks", [(1100, 1 << 30, 0), (300, 1 << 30, 0), (1100, 150, 40), (17, 600, 1)])
+def test_window_attention_long_padding(dev, sq, window, sinks, D):
+    """Masked keys of many tiles before, behind and between the others."""
+    sk = 1100
+    q, k, v = rnd(dev, 6, sq, 4, D), rnd(dev, 6, sk, 2, D, seed=1), rnd(dev, 6, sk, 2, D, seed=2)
+    mask = torch.zeros(6, sk, device=dev)
+    mask[0, 700:] = mask[1, :310] = mask[2, 1033] = mask[3, 0] = mask[4, 32:64] = mask[4, 600:608] = mask[4, 1099] = 1
+    k[mask == 0] = float("nan")
+    v[mask == 0] = float("inf")
+    check(Fn.window_attention(q, k, v, window, sinks, mask), *window_ref(q, k, v, window, sinks, mask))
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("sq,sk,D,G", [(1, 200, 128, 4), (3, 200, 64, 2), (64, 64, 64, 1), (150, 333, 128, 2)])
 def test_window_attention_hidden_keys_may_hold_anything(dev, bad, sq, sk, D, G):
