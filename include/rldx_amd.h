@@ -924,15 +924,18 @@ hipError_t rldx_rope_interleaved_f32(const float* xq, const int64_t* q_strides, 
  * seq_k <= 2^30) and sees key j iff
  *   j <= p  and  (j > p - window  or  j < sinks)  and  key_mask[b, j] != 0.
  * o = softmax over the visible keys of (q . k scale), times V; a query that sees
- * no key gets zeros.  A key that a query does not see has no influence on it,
- * whatever its K and V rows hold.  Query head h reads KV head h / (Hq / Hkv).
+ * no key (or whose scores are all -infinity) gets zeros.  A key that a query does
+ * not see has no influence on it, whatever its K and V rows hold.  Query head h
+ * reads KV head h / (Hq / Hkv).  B, Hq <= 65535, seq_q Hq / Hkv <= 2^30.
  *   q, o [B, seq_q, Hq, D], k, v [B, seq_k, Hkv, D]: strides {batch, seq, head}
- *   (3 int64 each, multiples of 8; D contiguous, 64 or 128), 16-byte aligned.
+ *   (3 int64 each, multiples of 8; D contiguous, 64 or 128; the seq strides of k
+ *   and v in [0, 2^24]), 16-byte aligned.
  *   key_mask: NULL, or fp32 [B, seq_k] (row stride key_mask_batch_stride, 0 =
  *   one row for every sequence), 4-byte aligned.  window >= 1, sinks >= 0.
  * workspace: >= rldx_window_attention_workspace_bytes(...) bytes, 16-byte
  * aligned, caller-owned (0 bytes: may be NULL), used until the call's launches
- * have run.  One launch, or two where few query rows split the keys.
+ * have run.  One launch, or two where the keys of few query rows are shared out;
+ * the sizes alone decide.
  *
  * No counterpart in the reference: the backbone's causal prefill
  *   (rldx/inference/backbone/llm/engine/kernels/fused_llm_attention.py:379-770)
@@ -958,12 +961,13 @@ int64_t rldx_window_attention_workspace_bytes(int64_t batch, int64_t q_heads, in
  * csrc/kv4_cache.h).  Slot s of sequence b is slot s % page_tokens of page
  * page_table[b][s / page_tokens].  Page ids are read on the device: an id outside
  * [0, num_pages) is a missing page, and so is a slot at or past table_pages *
- * page_tokens.  Nothing is read or written through a missing page.
+ * page_tokens.  Nothing is read or written through a missing page.  Scale bytes 0,
+ * 1, 253 and 254, which the append never writes, are not part of the format.
  */
 typedef struct rldx_kv4_cache {
   void* data;                /* pages, 16-byte aligned                                            */
   int64_t num_pages;         /* < 2^31                                                            */
-  int64_t kv_heads;
+  int64_t kv_heads;          /* <= 65535                                                          */
   int64_t head_dim;          /* 64 or 128                                                         */
   int64_t page_tokens;       /* power of two, 32 .. 2^20                                          */
   int64_t page_stride;       /* bytes, multiple of 16                                             */
@@ -992,7 +996,7 @@ int rldx_host_kv4_encode_bf16(const void* x, void* codes, void* scales, int64_t 
  * the nearest, ties to the even code, larger ones to 6, signs kept.  A block with
  * an infinity or a NaN reads back as NaN.  Slots below 0 and slots of missing
  * pages are skipped.  Two rows of one call must not write the same slot.
- * One launch, no workspace.
+ * batch <= 65535, seq <= 2^28.  One launch, no workspace.
  * No counterpart in the reference, which keeps no K/V between calls.
  */
 hipError_t rldx_kv4_append_bf16(const rldx_kv4_cache_t* cache, const void* k, const int64_t* k_strides,
@@ -1003,7 +1007,7 @@ hipError_t rldx_kv4_append_bf16(const rldx_kv4_cache_t* cache, const void* k, co
  * The values that the slots starts[b] .. starts[b] + seq - 1 hold, as bf16 rows
  * k, v [batch, seq, kv_heads, D] (layout as above; exact); a slot below 0 or of a
  * missing page gives NaN.  A slot that nobody has written gives whatever its
- * bytes stand for.  One launch, no workspace.
+ * bytes stand for.  batch <= 65535, seq <= 2^28.  One launch, no workspace.
  * No counterpart in the reference.
  */
 hipError_t rldx_kv4_read_bf16(const rldx_kv4_cache_t* cache, const int32_t* starts, void* k,
@@ -1019,7 +1023,7 @@ hipError_t rldx_kv4_read_bf16(const rldx_kv4_cache_t* cache, const int32_t* star
  * get zeros.  A query that sees a slot of a missing page gets NaN; pages whose
  * slots no query sees are not touched (a sliding window may give them back).
  * Slots that a query does not see have no influence on it, whatever they hold.
- * The products are those of the exact bf16 values, fp32 scores, softmax and sums.
+ * batch, Hq <= 65535, seq_q Hq / kv_heads <= 2^30.  The products are those of the exact bf16 values, fp32 scores, softmax and sums.
  * workspace: >= rldx_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned,
  * caller-owned (0 bytes: may be NULL), used until the call's launches have run.
  * One or two launches, which depend on the sizes alone: starts, counts and the

@@ -576,9 +576,10 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_attn_kernel(StreamArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Many query rows: 128 (token, head) rows of a KV head's group per workgroup, 32 a wave, and tiles of 32
-// keys that the workgroup brings into LDS once: bf16 rows straight from memory (buffer_load ... lds, three slots
-// ahead of the matrix work), codes of the cache through registers, as the bf16 values they stand for.
+// Many query rows: 32 (token, head) rows of a KV head's group a wave, and tiles of 32 keys that the workgroup brings into
+// LDS once, NG of them a step: bf16 rows straight from memory (buffer_load ... lds, up to two slots ahead of the matrix
+// work), codes of the cache through registers, as the bf16 values they stand for.  The NW waves are NW / NG blocks of 32
+// rows times NG key groups, which take a tile of the step each and add up their states at the end.
 //   S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16_bf16: a lane owns a query column, so maxima, sums and
 //   rescaling stay in the lane and its partner (lane ^ 32), and P^T goes from accumulator to operand in place.
 //   Both operands lie in LDS as rows, 16-byte pieces of row r exchanged by an XOR: K's by r mod the pieces of a row
@@ -586,6 +587,10 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_attn_kernel(StreamArgs a) {
 //   gathers 4 keys of 16 dimensions, 32 bytes of each of 4 rows, into the V^T operand).
 // Rows in (token, head) order keep the workgroup's windows together: 128 rows of 4 heads a group span 32 tokens, so
 // a window of 1024 takes 34 tiles of which every wave needs 33.
+// Bound: a step of 128 rows and 32 keys costs a CU 0.6 us with three workgroups on it, 0.2 of them matrix instructions at
+// their peak rate, most of the rest the softmax's vector work (8192 tokens of 32/8 heads of 128, window 1024: 162 us, 0.80
+// PFLOP/s of what is seen; 4096 causal tokens: 146 us, 0.94, where a loop of nothing but the reads and products of such
+// tiles ends at 1.14); 1 us where a workgroup has the CU for itself: LDS reads, products and softmax in a chain.
 // ---------------------------------------------------------------------------
 template <int N>
 __device__ __forceinline__ void vm_wait_barrier() {  // all but this wave's last N loads have arrived, everywhere
@@ -1245,7 +1250,7 @@ bool a16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 struct Plan {
   int waves;                  // of a workgroup: 4 or 8
   int rb, row_tiles, splits;  // rows of a workgroup: 16 (rows_attn_kernel), 32, 64 or 128 (tile_attn_kernel)
-  int64_t items;  // row blocks times splits
+  int64_t items;              // row blocks times splits
   int64_t workspace(int64_t head_dim) const { return splits > 1 ? items * rb * (head_dim + 2) * 4 : 0; }
 };
 
@@ -1253,7 +1258,8 @@ struct Plan {
 bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t seq_q, int64_t limit, int64_t head_dim,
              int64_t window, int64_t sinks, bool cache) {
   if ((head_dim != 64 && head_dim != 128) || batch < 0 || q_heads < 0 || kv_heads <= 0 || q_heads % kv_heads ||
-      seq_q < 0 || limit < 0 || limit > kMaxSlots || window < 1 || sinks < 0 || batch > 65535 || q_heads > 65535)
+      seq_q < 0 || limit < 0 || limit > kMaxSlots || window < 1 || sinks < 0 || batch > 65535 || q_heads > 65535 ||
+      kv_heads > 65535)
     return false;
   const int64_t group = q_heads / kv_heads, rows = seq_q * group;
   if (seq_q > kMaxSlots || rows > kMaxSlots) return false;
@@ -1306,7 +1312,8 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     if (more <= (!cache && head_dim == 128 ? 0 : 2)) p.waves = 8, p.splits = 1;
   }
   p.items = blocks * p.splits;
-  return p.items <= (int64_t{1} << 31) - 1 && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
+  // (threads of a grid: 32 bits)
+  return p.items * 64 * p.waves < (int64_t{1} << 32) && batch * q_heads * seq_q <= (int64_t{1} << 31) - 1;
 }
 
 bool strides_ok(const int64_t* s) { return s && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0; }

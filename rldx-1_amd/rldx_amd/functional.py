@@ -566,6 +566,14 @@ def llm_fused_attention(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: tor
 NO_WINDOW = 1 << 30  # a window that holds every slot there can be
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def _device_of(t: torch.Tensor):
+    """t's device made the current one: a default stream is that of the current device."""
+    return _SAME_DEVICE if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def _rows4(t: torch.Tensor, what: str):
     """Strides {batch, seq, head} of a bf16 [B, S, H, D] (0 for a dimension of one: it is never stepped over)."""
     _require(t.dtype == BF16 and t.dim() == 4, f"{what} must be bf16 [B, S, H, D]")
@@ -607,6 +615,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     _require(k.shape[0] == B and k.shape[3] == D and v.shape == k.shape, "k and v must be [B, Sk, Hkv, D] matching q")
     _require(Hkv > 0 and Hq % Hkv == 0, "q heads must be a multiple of kv heads")
     _require(Sq <= Sk, "the queries are the last of the keys: Sq <= Sk")
+    _require(max(ks[1], vs[1]) <= 1 << 24, "k and v: at most 2^24 elements from token to token")
     window, sinks = int(window), int(sinks)
     _require(window >= 1 and sinks >= 0, "window must be at least 1, sinks at least 0")
     mp, ms = None, 0
@@ -622,11 +631,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         return out
     lib = _lib.load()
     need = int(lib.rldx_window_attention_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, window, sinks))
-    _require(need >= 0, "window_attention: sizes out of range (Sk and Sq * Hq / Hkv up to 2^30)")
+    _require(need >= 0, "window_attention: sizes out of range (B and Hq up to 65535, Sk and Sq * Hq / Hkv up to 2^30)")
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.check(lib.rldx_window_attention_bf16(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os_,
-                                              B, Hq, Hkv, Sq, Sk, D, window, sinks, mp, ms, scale, _ptr(ws), need,
-                                              _stream_ptr(q)), "rldx_window_attention_bf16")
+    with _device_of(q):
+        _lib.check(lib.rldx_window_attention_bf16(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
+                                                  os_, B, Hq, Hkv, Sq, Sk, D, window, sinks, mp, ms, scale, _ptr(ws),
+                                                  need, _stream_ptr(q)), "rldx_window_attention_bf16")
     return out
 
 
@@ -672,9 +682,11 @@ def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page_table
     c = _kv4(cache, page_table, starts, counts, B, H, D)
     if k.numel() == 0:
         return
+    _require(B <= 65535 and S <= 1 << 28, "kv4_append: at most 65535 sequences and 2^28 rows of each")
     lib = _lib.load()
-    _lib.check(lib.rldx_kv4_append_bf16(c, k.data_ptr(), ks, v.data_ptr(), vs, starts.data_ptr(), _ptr(counts), B, S,
-                                        _stream_ptr(k)), "rldx_kv4_append_bf16")
+    with _device_of(k):
+        _lib.check(lib.rldx_kv4_append_bf16(c, k.data_ptr(), ks, v.data_ptr(), vs, starts.data_ptr(), _ptr(counts), B, S,
+                                            _stream_ptr(k)), "rldx_kv4_append_bf16")
 
 
 def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor, count: int, head_dim: int):
@@ -683,6 +695,7 @@ def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor
     _on_gpu(cache, page_table, starts)
     _require(starts.dim() == 1 and count >= 0, "starts must be int32 [B], count at least 0")
     B = starts.shape[0]
+    _require(B <= 65535 and count <= 1 << 28, "kv4_read: at most 65535 sequences and 2^28 rows of each")
     c = _kv4(cache, page_table, starts, None, B, None, head_dim)
     k = torch.empty((B, count, cache.shape[1], head_dim), dtype=BF16, device=cache.device)
     v = torch.empty_like(k)
@@ -690,8 +703,9 @@ def kv4_read(cache: torch.Tensor, page_table: torch.Tensor, starts: torch.Tensor
         return k, v
     lib = _lib.load()
     st = _rows4(k, "k")
-    _lib.check(lib.rldx_kv4_read_bf16(c, starts.data_ptr(), k.data_ptr(), st, v.data_ptr(), st, B, count, _stream_ptr(k)),
-               "rldx_kv4_read_bf16")
+    with _device_of(k):
+        _lib.check(lib.rldx_kv4_read_bf16(c, starts.data_ptr(), k.data_ptr(), st, v.data_ptr(), st, B, count,
+                                          _stream_ptr(k)), "rldx_kv4_read_bf16")
     return k, v
 
 
@@ -717,11 +731,12 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor
         return out
     lib = _lib.load()
     need = int(lib.rldx_kv4_attention_workspace_bytes(B, Hq, Hkv, Sq, D, c.page_tokens, c.table_pages, window, sinks))
-    _require(need >= 0, "kv4_attention: sizes out of range (Sq * Hq / Hkv up to 2^30)")
+    _require(need >= 0, "kv4_attention: sizes out of range (B and Hq up to 65535, Sq * Hq / Hkv up to 2^30)")
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.check(lib.rldx_kv4_attention_bf16(q.data_ptr(), qs, c, starts.data_ptr(), _ptr(counts), out.data_ptr(), os_, B,
-                                           Hq, Sq, window, sinks, scale, _ptr(ws), need, _stream_ptr(q)),
-               "rldx_kv4_attention_bf16")
+    with _device_of(q):
+        _lib.check(lib.rldx_kv4_attention_bf16(q.data_ptr(), qs, c, starts.data_ptr(), _ptr(counts), out.data_ptr(), os_,
+                                               B, Hq, Sq, window, sinks, scale, _ptr(ws), need, _stream_ptr(q)),
+                   "rldx_kv4_attention_bf16")
     return out
 
 

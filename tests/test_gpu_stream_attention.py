@@ -547,6 +547,39 @@ def _stream_step(c, table, starts, q, k, v):
     return torch.ops.rldx_amd.kv4_attention(q, c, table, starts, None, 2000, 4)
 
 
+def test_refused_token_strides(dev):
+    wide = torch.empty((1 << 24) + 8 + 64, dtype=torch.bfloat16, device=dev).as_strided((1, 2, 1, 64), (0, (1 << 24) + 8, 64, 1))
+    q, k = rnd(dev, 1, 2, 1, 64), rnd(dev, 1, 2, 1, 64)
+    for args in ((q, wide, k, 4), (q, k, wide, 4)):
+        with pytest.raises(RuntimeError, match="from token to token"):
+            torch.ops.rldx_amd.window_attention(*args)
+
+
+def test_tensors_off_the_current_device(dev, monkeypatch):
+    """The launchers make the tensors' device the current one where it is not."""
+    q, k = rnd(dev, 1, 4, 4, 64), rnd(dev, 1, 40, 2, 64)
+    c, table = cache_of(dev, 1, 64, 2, 64, 32)
+    st = ints(dev, 3)
+
+    def calls():
+        Fn.kv4_append(c, k, k, table, ints(dev, 0))
+        return (Fn.window_attention(q, k, k, 9), *Fn.kv4_read(c, table, st, 30, 64), Fn.kv4_attention(q, c, table, st))
+
+    class Entered(torch.cuda.device):
+        at = []
+
+        def __enter__(self):
+            self.at.append(self.idx)
+            return super().__enter__()
+
+    want = calls()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", Entered)
+    got = calls()
+    monkeypatch.undo()
+    assert Entered.at == [0] * 4 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_two_streams_at_once(dev):
     """Calls on two streams, nothing waiting between them: each has a workspace of its own."""
     sets = []

@@ -174,3 +174,18 @@ def test_fakes():
     assert o.shape == q.shape and o.is_contiguous() and o.dtype == BF16
     assert rk.shape == rv.shape == (2, 7, 2, 128) and rk.dtype == BF16
     assert a.shape == q.shape and a.dtype == BF16
+
+
+def test_abi_refuses_sizes_that_the_kernels_do_not_address():
+    lib = _lib.load()
+    st = _lib.i64_array([8192, 256, 128])
+    for seq in (-256, (1 << 24) + 8):
+        bad = _lib.i64_array([8192, seq, 128])
+        for ks, vs in ((bad, st), (st, bad)):
+            assert lib.rldx_window_attention_bf16(P, st, P, ks, P, vs, P, st, 1, 2, 2, 4, 64, 128, 16, 0, None, 0, 0.1, None, 0,
+                                                  None) == INVALID
+    assert lib.rldx_kv4_append_bf16(_cache(), P, st, P, st, P, None, 1, (1 << 28) + 1, None) == INVALID
+    assert lib.rldx_kv4_read_bf16(_cache(), P, P, st, P, st, 1, (1 << 28) + 1, None) == INVALID
+    # more threads than a grid has
+    assert lib.rldx_window_attention_workspace_bytes(1 << 15, 1 << 13, 1 << 13, 1, 40, 64, 8, 0) == -1
+    assert lib.rldx_window_attention_workspace_bytes(1 << 15, 1 << 8, 1 << 8, 1, 40, 64, 8, 0) == 0
