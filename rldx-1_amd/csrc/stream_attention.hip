@@ -651,9 +651,10 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   constexpr int NS = kCache || NG > 1 ? 2 : 3;  // ring slots
   constexpr int OP = D + 8;              // pitch of O rows staged in LDS
   constexpr int RING = NS * NG * TILEB, STAGE = NW * 32 * OP * 2;
-  constexpr int FT = 4 * NG / NW;        // cache: tiles of a step that 4 waves turn into values
+  constexpr int FT = 4 * NG / NW;        // tiles of a step that 4 waves bring
+  static_assert(FT == NG || FT == 1 || kCache, "a group of 4 waves walks one tile of a step");
   static_assert(NG == 1 || NG == 2 || NG == 4, "key groups");
-  static_assert(NW == kWaves || (kCache && NW == 8 && NG > 1), "waves");
+  static_assert(NW == kWaves || (NW == 8 && NG > 1), "waves");
   constexpr int EXCH = NG > 1 ? NW * (DBLK * 4 + 1) * 1024 : 0;  // states that the key groups exchange
   constexpr int LDS = RING > STAGE ? (RING > EXCH ? RING : EXCH) : (STAGE > EXCH ? STAGE : EXCH);
   __shared__ __attribute__((aligned(1024))) uint8_t ring[LDS];
@@ -717,7 +718,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   int drow[CPW], dk[CPW], dv[CPW];
 #pragma unroll
   for (int c = 0; c < CPW; ++c) {
-    drow[c] = (wave + kWaves * c) * (1024 / ROWB) + lane / PCS;
+    drow[c] = (wave % 4 + 4 * c) * (1024 / ROWB) + lane / PCS;
     dk[c] = drow[c] * static_cast<int>(a.k_ss * 2) + ((lane % PCS) ^ swz_k(drow[c])) * 16;
     dv[c] = drow[c] * static_cast<int>(a.v_ss * 2) + ((lane % PCS) ^ swz_v(drow[c])) * 16;
   }
@@ -732,7 +733,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   };
   auto dma = [&](int off) {
     const int k0 = d_tile * kTile;
-    uint8_t* const to = ring + off + wave * 1024;
+    uint8_t* const to = ring + off + wave % 4 * 1024;
     int ok[CPW], ov[CPW];
 #pragma unroll
     for (int c = 0; c < CPW; ++c) ok[c] = dk[c], ov[c] = dv[c];
@@ -745,10 +746,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
       }
     }
 #pragma unroll
-    for (int c = 0; c < CPW; ++c) load_lds16(kt, to + kWaves * c * 1024, ok[c]);
+    for (int c = 0; c < CPW; ++c) load_lds16(kt, to + 4 * c * 1024, ok[c]);
 #pragma unroll
-    for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + kWaves * c * 1024, ov[c]);
-    if (++d_it < n) {
+    for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + 4 * c * 1024, ov[c]);
+    if constexpr (FT < NG) {
+      d_it += NG;  // (FT = 1)
+      dma_seek(tile_at(d_it));
+    } else if (++d_it < n) {
       if (d_tile + 1 == sp.ns) {
         dma_seek(sp.w0);
       } else {
@@ -1012,15 +1016,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
     } else {
       auto dma_step = [&](int slot) {
 #pragma unroll
-        for (int x = 0; x < NG; ++x) dma((slot * NG + x) * TILEB);
+        for (int x = 0; x < FT; ++x) dma((slot * NG + fg * FT + x) * TILEB);
       };
       fetch_mask(kg);
-      dma_seek(tile_at(0));
+      d_it = FT < NG ? fg : 0;
+      dma_seek(tile_at(d_it));
 #pragma unroll
       for (int x = 0; x < NS - 1; ++x) dma_step(x);
       int slot = 0;
       for (int st = 0; st < steps; ++st) {
-        vm_wait_barrier<(NS - 2) * NG * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
+        vm_wait_barrier<(NS - 2) * FT * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
         uint32_t mask = ~0u;
         if constexpr (kMask) mask = static_cast<uint32_t>(__ballot(mload != 0.f));
         fetch_mask((st + 1) * NG + kg);
@@ -1308,9 +1313,19 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     // us, 516 with 8 waves; 1024 tokens, which do, 246 and 172).
     if (p.rb == 64 || (p.rb == 128 && heads * row_tiles(128) <= per_cu * cus)) p.waves = 8;
   } else {
-    // The smallest row blocks whose workgroups run all at once, else 128 rows.  us for 32 / 64 / 128 rows, window: 169
-    // queries of 28/4 heads of 128 17 / 25 / 29, 640 of them 29 / 19 / 23, 8192 of 32/8 heads 443 / 223 / 172.
-    p.rb = heads * row_tiles(32) <= per_cu * cus ? 32 : heads * row_tiles(64) <= 2 * per_cu * cus ? 64 : 128;
+    // The smallest row blocks whose workgroups run all at once, else 128 rows by 4 waves (us for 32 / 64 / 128 rows of 28/4
+    // heads of 128: 169 queries over 1449 keys 16 / 19 / 22, 640 x 640 26 / 16 / 22, 1280 x 1280, window 512, 50 / 32 / 28).
+    // But each block reads its keys again, and few blocks share them out: over long ranges 64 rows (169 x 3000 34 / 26 /
+    // 29), then 128 by 8 waves, two tiles a step (for 32 / 64 / these: 169 x 8192 78 / 47 / 36, 300 x 8192 147 / 106 / 57;
+    // 300 x 1449 29 / 21 / 25).  head_dim 64 with two workgroups of 32 rows on most CUs: 512 x 4096 of 32/8 heads 34 / 45 / 41.
+    const int64_t blocks32 = heads * row_tiles(32), blocks64 = heads * row_tiles(64), steps32 = steps_of(32, 4);
+    if (blocks32 <= per_cu * cus && (steps32 <= 16 || (blocks32 > cus && steps32 <= 64)))
+      p.rb = 32;
+    else if (blocks64 <= 2 * per_cu * cus && !(blocks64 <= cus && steps_of(64, 2) > 20))
+      p.rb = 64;
+    else
+      p.rb = 128;
+    if (p.rb == 128 && blocks64 <= cus) p.waves = 8;
   }
   p.row_tiles = static_cast<int>(row_tiles(p.rb));
   const int64_t blocks = heads * p.row_tiles, tiles = tiles_of(p.rb);
@@ -1384,10 +1399,10 @@ hipError_t launch(const StreamArgs& a, const Plan& p, hipStream_t stream) {
     else
       launch_tiles<D, 2, false, 4>(a, grid, stream);
   } else {
-    bool taken = false;
-    if constexpr (kCache)
-      if ((taken = p.waves == 8)) launch_tiles<D, 2, true, 8>(a, grid, stream);
-    if (!taken) launch_tiles<D, 1, kCache, 4>(a, grid, stream);
+    if (p.waves == 8)
+      launch_tiles<D, 2, kCache, 8>(a, grid, stream);
+    else
+      launch_tiles<D, 1, kCache, 4>(a, grid, stream);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;

@@ -110,6 +110,21 @@ def test_window_attention_key_mask(dev, sq, sk, D, Hq, Hkv):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", [(1, 300, 2500, 28, 4), (2, 49, 6000, 28, 4), (1, 500, 2049, 16, 16), (1, 41, 9000, 64, 2)], ids=str)
+def test_window_attention_long_chunks(dev, case, D):
+    """Chunks behind long pasts, with values that only some queries may see and a key mask."""
+    B, sq, sk, Hq, Hkv = case
+    q, k, v = rnd(dev, B, sq, Hq, D), rnd(dev, B, sk, Hkv, D, seed=1), rnd(dev, B, sk, Hkv, D, seed=2)
+    check(Fn.window_attention(q, k, v, 1 << 30), *window_ref(q, k, v, 1 << 30, 0), "whole")
+    mask = (torch.rand(B, sk, generator=torch.Generator().manual_seed(5)) < 0.9).float().to(dev)
+    mask[-1, :800] = 0
+    k[mask == 0], v[mask == 0] = float("nan"), float("inf")
+    check(Fn.window_attention(q, k, v, 1700, 40, mask), *window_ref(q, k, v, 1700, 40, mask), "mask")
+    v[:, sk - 3, 0, 5], v[:, sk - sq // 2, Hkv - 1, D - 1] = float("inf"), float("nan")
+    check(Fn.window_attention(q, k, v, 1700, 40, mask), *window_ref(q, k, v, 1700, 40, mask), "infinite")
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("sq,window,sinks", [(1100, 1 << 30, 0), (300, 1 << 30, 0), (1100, 150, 40), (17, 600, 1)])
 def test_window_attention_long_padding(dev, sq, window, sinks, D):
     """Masked keys of many tiles before, behind and between the others."""
