@@ -1184,6 +1184,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   }
 }
 
+// x of the lane y further round in this lane's 16
+__device__ __forceinline__ float row_turned(float x, int y) {
+  const int b = __builtin_bit_cast(int, x);
+  const int r = y == 1 ? __builtin_amdgcn_mov_dpp(b, 0x121, 0xf, 0xf, false)
+              : y == 2 ? __builtin_amdgcn_mov_dpp(b, 0x122, 0xf, 0xf, false)
+              : y == 4 ? __builtin_amdgcn_mov_dpp(b, 0x124, 0xf, 0xf, false)
+                       : __builtin_amdgcn_mov_dpp(b, 0x128, 0xf, 0xf, false);
+  return __builtin_bit_cast(float, r);
+}
+
 // O of the query rows from the partial states of their splits: `per` waves (1 up to 16 splits, else 4) to a row, wave w
 // of them adds up splits w, w + per, ... .  Every state is loaded before anything is known about its use: one round trip
 // through memory, whichever of the splits had tiles.
@@ -1223,11 +1233,13 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(StreamArgs a, int rb
   m = lane < use ? m : -__builtin_inff();
   float top = m;
 #pragma unroll
-  for (int y = 1; y < 64; y *= 2) top = fmaxf(top, __shfl_xor(top, y));
+  for (int y = 1; y < 16; y *= 2) top = fmaxf(top, row_turned(top, y));
+  top = quad_max(top);
   const float w = rescale(m, top);
   l = lane < use ? l * w : 0.f;
 #pragma unroll
-  for (int y = 1; y < 64; y *= 2) l += __shfl_xor(l, y);
+  for (int y = 1; y < 16; y *= 2) l += row_turned(l, y);
+  l = quad_sum(l);
   float acc[E] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -1330,6 +1342,10 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
   p.row_tiles = static_cast<int>(row_tiles(p.rb));
   const int64_t blocks = heads * p.row_tiles, tiles = tiles_of(p.rb);
   p.splits = static_cast<int>(splits_for(blocks, tiles, (p.rb == kRowsBlock ? 2 : 1) * cus));
+  // (two workgroups of 8 waves to a CU, of head_dim 64, where each has tiles enough: 169 tokens of 28/4 heads over 20000 slots
+  // 63 -> 53 us, 300 over 8192 keys 43 -> 37; 2 x 49 over 6000 slots, 19 tiles each, 22 -> 27)
+  if (p.rb == 128 && p.waves == 8 && head_dim == 64 && tiles >= 40 * p.splits)
+    p.splits = static_cast<int>(splits_for(blocks, tiles, 2 * cus));
   // Sharing a row block out means a second launch, about 3 us.  Where 8 waves walk the tiles in (nearly) as few steps as
   // 4 waves of each split do, one workgroup of 8 takes the row block whole.  A step takes a workgroup 0.5 us (codes,
   // head_dim 64), 0.9 (codes, or rows of 64) or 1.7 (rows of 128, 128 KB).  Token of 32/8 heads of 128, shared out ->
@@ -1337,7 +1353,10 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
   // 7.9 -> 6.1, 500 keys 7.9 (8.6 whole), 32 sequences of 1000 keys 29.3 -> 25.9.
   if (p.rb == kRowsBlock && p.splits > 1) {
     const int64_t more = (tiles + 7) / 8 - (tiles + 4 * p.splits - 1) / (4 * p.splits);
-    if (more <= (!cache && head_dim == 128 ? 0 : 2)) p.waves = 8, p.splits = 1;
+    if (more <= (!cache && head_dim == 128 ? 0 : 2))
+      p.waves = 8, p.splits = 1;
+    else if (head_dim == 64)  // three workgroups of 4 waves on a CU: 16 x 8000 keys of 24/8 heads 59 -> 54 us, slots 20.3 -> 19.4
+      p.splits = static_cast<int>(splits_for(blocks, tiles, 3 * cus));
   }
   p.items = blocks * p.splits;
   // (threads of a grid: 32 bits)
