@@ -781,14 +781,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
     return a.cache + page * a.page_stride + hk * a.head_stride +
            (((tile_at(it) * kTile) & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
   };
-  // threads 0 .. 127 take K, D / 4 dimensions of a row each, the others V, a quarter of the lane blocks' units
+  // Threads 0 .. 127 of a group of 4 waves take K, D / 4 dimensions of a row each, the others V, half of a lane's units
+  // (16 lanes next to each other: what they write at once lies in different banks).
   const int ct = static_cast<int>(threadIdx.x) & 127;
   auto fetch = [&](int page, int it, u32x4& codes, uint32_t& scales) {
     codes = u32x4{0, 0, 0, 0};
     scales = 0;
     if (page < 0) return;
     const uint8_t* const t = tile_ptr(page, it);
-    const uint8_t* const src = t + ((wave & 3) < 2 ? 0 : 16 * D) + ct * (D / 8);
+    const int half = ct >> 4 & 1, lb = ct >> 5 << 4 | (ct & 15);
+    const uint8_t* const src = t + ((wave & 3) < 2 ? ct * (D / 8) : 16 * D + (2 * lb + half) * (D / 8));
     if constexpr (D == 128) {
       codes = *reinterpret_cast<const u32x4*>(src);
     } else {
@@ -798,8 +800,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
     if ((wave & 3) < 2) {
       scales = t[32 * D + (ct >> 2) * (D / 32) + (D == 128 ? ct & 3 : (ct & 3) >> 1)];
     } else {  // the scales of 4 slots
-      const int lb = ct >> 1;
-      scales = *reinterpret_cast<const uint32_t*>(t + 33 * D + ((lb & 15) * (D / 16) / 32 * 4 + (lb >> 4)) * 8 + (ct & 1) * 4);
+      scales = *reinterpret_cast<const uint32_t*>(t + 33 * D + ((lb & 15) * (D / 16) / 32 * 4 + (lb >> 4)) * 8 + half * 4);
     }
   };
   auto store = [&](int off, u32x4 codes, uint32_t scales) {
@@ -814,8 +815,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
         *reinterpret_cast<bf16x8*>(ks + r * ROWB + (piece ^ swz_k(r)) * 16) = dequant8(c, sc);
       }
     } else {
-      const int lb = ct >> 1;
-      const int r0 = 16 * (ct & 1) + 4 * (lb >> 4), col = lb & 15;
+      const int r0 = 16 * (ct >> 4 & 1) + 4 * (ct >> 5), col = ct & 15;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = r0 + j;
