@@ -646,13 +646,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   constexpr int PCS = D / 8;       // 16-byte pieces of a row
   constexpr int ROWB = 2 * D;      // bytes of a row
   constexpr int CH = 32 * ROWB / 1024;   // 1 KB chunks of a tile's K or V
-  constexpr int CPW = CH / kWaves;       // of them a wave loads (D = 64: one)
+  constexpr int CPW = CH / NQ;           // of them a wave loads: the waves of a key group bring its tile
   constexpr int TILEB = 2 * 32 * ROWB;   // K and V of a tile in LDS; a ring slot holds NG tiles, a step's
   constexpr int NS = kCache || NG > 1 ? 2 : 3;  // ring slots
   constexpr int OP = D + 8;              // pitch of O rows staged in LDS
   constexpr int RING = NS * NG * TILEB, STAGE = NW * 32 * OP * 2;
-  constexpr int FT = 4 * NG / NW;        // tiles of a step that 4 waves bring
-  static_assert(FT == NG || FT == 1 || kCache, "a group of 4 waves walks one tile of a step");
   static_assert(NG == 1 || NG == 2 || NG == 4, "key groups");
   static_assert(NW == kWaves || (NW == 8 && NG > 1), "waves");
   constexpr int EXCH = NG > 1 ? NW * (DBLK * 4 + 1) * 1024 : 0;  // states that the key groups exchange
@@ -661,7 +659,6 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
   const int l32 = lane & 31, g = lane >> 5;
-  const int fg = wave / 4;
   const int wq = wave % NQ, kg = wave / NQ;  // the wave's block of 32 rows, and its share of the tiles
 
   // Work item: (batch, kv head, row tile, split).  Workgroup i runs on XCD i % 8: the items of a pair (batch, kv head),
@@ -718,7 +715,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   int drow[CPW], dk[CPW], dv[CPW];
 #pragma unroll
   for (int c = 0; c < CPW; ++c) {
-    drow[c] = (wave % 4 + 4 * c) * (1024 / ROWB) + lane / PCS;
+    drow[c] = (wq + NQ * c) * (1024 / ROWB) + lane / PCS;
     dk[c] = drow[c] * static_cast<int>(a.k_ss * 2) + ((lane % PCS) ^ swz_k(drow[c])) * 16;
     dv[c] = drow[c] * static_cast<int>(a.v_ss * 2) + ((lane % PCS) ^ swz_v(drow[c])) * 16;
   }
@@ -733,7 +730,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
   };
   auto dma = [&](int off) {
     const int k0 = d_tile * kTile;
-    uint8_t* const to = ring + off + wave % 4 * 1024;
+    uint8_t* const to = ring + off + wq * 1024;
     int ok[CPW], ov[CPW];
 #pragma unroll
     for (int c = 0; c < CPW; ++c) ok[c] = dk[c], ov[c] = dv[c];
@@ -746,11 +743,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
       }
     }
 #pragma unroll
-    for (int c = 0; c < CPW; ++c) load_lds16(kt, to + 4 * c * 1024, ok[c]);
+    for (int c = 0; c < CPW; ++c) load_lds16(kt, to + NQ * c * 1024, ok[c]);
 #pragma unroll
-    for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + 4 * c * 1024, ov[c]);
-    if constexpr (FT < NG) {
-      d_it += NG;  // (FT = 1)
+    for (int c = 0; c < CPW; ++c) load_lds16(vt, to + 32 * ROWB + NQ * c * 1024, ov[c]);
+    if constexpr (NG > 1) {
+      d_it += NG;
       dma_seek(tile_at(d_it));
     } else if (++d_it < n) {
       if (d_tile + 1 == sp.ns) {
@@ -781,31 +778,31 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
     return a.cache + page * a.page_stride + hk * a.head_stride +
            (((tile_at(it) * kTile) & ((1 << a.page_shift) - 1)) / kTile) * kv4::tile_bytes(D);
   };
-  // Threads 0 .. 127 of a group of 4 waves take K, D / 4 dimensions of a row each, the others V, half of a lane's units
-  // (16 lanes next to each other: what they write at once lies in different banks).
-  const int ct = static_cast<int>(threadIdx.x) & 127;
-  auto fetch = [&](int page, int it, u32x4& codes, uint32_t& scales) {
+  // A tile in 256 shares, 64 a wave at a time: part 0 and 1 are K's, D / 4 dimensions of a row each, 2 and 3 V's, half of a
+  // lane's units (16 lanes next to each other: what they write at once lies in different banks).
+  auto fetch = [&](int page, int it, int part, u32x4& codes, uint32_t& scales) {
     codes = u32x4{0, 0, 0, 0};
     scales = 0;
     if (page < 0) return;
     const uint8_t* const t = tile_ptr(page, it);
-    const int half = ct >> 4 & 1, lb = ct >> 5 << 4 | (ct & 15);
-    const uint8_t* const src = t + ((wave & 3) < 2 ? ct * (D / 8) : 16 * D + (2 * lb + half) * (D / 8));
+    const int ct = (part & 1) * 64 + lane, half = ct >> 4 & 1, lb = ct >> 5 << 4 | (ct & 15);
+    const uint8_t* const src = t + (part < 2 ? ct * (D / 8) : 16 * D + (2 * lb + half) * (D / 8));
     if constexpr (D == 128) {
       codes = *reinterpret_cast<const u32x4*>(src);
     } else {
       const u32x2 x = *reinterpret_cast<const u32x2*>(src);
       codes = u32x4{x[0], x[1], 0, 0};
     }
-    if ((wave & 3) < 2) {
+    if (part < 2) {
       scales = t[32 * D + (ct >> 2) * (D / 32) + (D == 128 ? ct & 3 : (ct & 3) >> 1)];
     } else {  // the scales of 4 slots
       scales = *reinterpret_cast<const uint32_t*>(t + 33 * D + ((lb & 15) * (D / 16) / 32 * 4 + (lb >> 4)) * 8 + half * 4);
     }
   };
-  auto store = [&](int off, u32x4 codes, uint32_t scales) {
+  auto store = [&](int off, int part, u32x4 codes, uint32_t scales) {
     uint8_t* const ks = ring + off;
-    if ((wave & 3) < 2) {
+    const int ct = (part & 1) * 64 + lane;
+    if (part < 2) {
       const int r = ct >> 2;
       const float sc = __builtin_bit_cast(float, scales << 23);
 #pragma unroll
@@ -985,28 +982,28 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
     const int steps = (n + NG - 1) / NG;
     if constexpr (kCache) {
       load_ids(0);
-      u32x4 codes[FT];
-      uint32_t scales[FT];
+      constexpr int PARTS = 4 / NQ;  // of its key group's tile a wave takes
+      u32x4 codes[PARTS];
+      uint32_t scales[PARTS];
       int own = -1, own_next = -1;  // the page of this wave's tile
       auto fetch_step = [&](int st) {
-        int mine = -1;
+        const int page = st * NG + kg < n ? page_of(st * NG + kg) : -1;
 #pragma unroll
-        for (int x = 0; x < FT; ++x) {
-          const int t = fg * FT + x, page = st * NG + t < n ? page_of(st * NG + t) : -1;
-          fetch(page, st * NG + t, codes[x], scales[x]);
-          mine = t == kg ? page : mine;
-        }
-        return mine;
+        for (int x = 0; x < PARTS; ++x) fetch(page, st * NG + kg, wq + NQ * x, codes[x], scales[x]);
+        return page;
       };
       auto store_step = [&](int slot) {
 #pragma unroll
-        for (int x = 0; x < FT; ++x) store((slot * NG + fg * FT + x) * TILEB, codes[x], scales[x]);
+        for (int x = 0; x < PARTS; ++x) store((slot * NG + kg) * TILEB, wq + NQ * x, codes[x], scales[x]);
       };
       own = fetch_step(0);
       store_step(0);
       if (steps > 1) own_next = fetch_step(1);
       for (int st = 0; st < steps; ++st) {
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if constexpr (NQ == 1)  // (a tile of one wave's own: what it wrote and read it has waited for itself)
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        else
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const int page = own;
         own = own_next;
         if (st + 1 < steps) store_step((st + 1) & 1);
@@ -1014,18 +1011,18 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
         if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, ((st & 1) * NG + kg) * TILEB, page, ~0u);
       }
     } else {
-      auto dma_step = [&](int slot) {
-#pragma unroll
-        for (int x = 0; x < FT; ++x) dma((slot * NG + fg * FT + x) * TILEB);
-      };
+      auto dma_step = [&](int slot) { dma((slot * NG + kg) * TILEB); };
       fetch_mask(kg);
-      d_it = FT < NG ? fg : 0;
+      d_it = kg;
       dma_seek(tile_at(d_it));
 #pragma unroll
       for (int x = 0; x < NS - 1; ++x) dma_step(x);
       int slot = 0;
       for (int st = 0; st < steps; ++st) {
-        vm_wait_barrier<(NS - 2) * FT * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
+        if constexpr (NQ == 1)  // (a tile of one wave's own)
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else
+          vm_wait_barrier<(NS - 2) * 2 * CPW>();  // the step's tiles are in LDS, the slot of the last step is free
         uint32_t mask = ~0u;
         if constexpr (kMask) mask = static_cast<uint32_t>(__ballot(mload != 0.f));
         fetch_mask((st + 1) * NG + kg);
