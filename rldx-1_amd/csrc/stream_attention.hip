@@ -163,16 +163,14 @@ __device__ __forceinline__ bf16x8 dequant8(uint32_t c, float s) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// (The pairs are opaque to the compiler in these, or it works them out ahead for every tile, and keeps registers for
-// them, though only a few tiles come here.)
-// Whether any of the bf16 values looked at is an infinity or a NaN: 0 times it is a NaN.
+// (The instructions of these are opaque to the compiler, or it works them out ahead for every tile, and keeps registers
+// for them, though only a few tiles come here.)
+// Whether any of the bf16 values looked at is an infinity or a NaN: 0 times it is a NaN.  Looked at as fp16 pairs, one
+// instruction for two: exponents from 0xf8 on count as well, values of 2^121 and more, which the caller tells apart.
 struct Finite {
-  float sum = 0.f;
-  __device__ __forceinline__ void look(uint32_t w) {
-    asm volatile("" : "+v"(w));
-    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), bf16x2_t{0, 0}, sum, false);
-  }
-  __device__ __forceinline__ bool broken() const { return sum != sum; }
+  uint32_t sum = 0;
+  __device__ __forceinline__ void look(uint32_t w) { asm volatile("v_pk_fma_f16 %0, %1, 0, %0" : "+v"(sum) : "v"(w)); }
+  __device__ __forceinline__ bool broken() const { return (sum & 0x7fffu) > 0x7c00u || (sum & 0x7fff0000u) > 0x7c000000u; }
 };
 __device__ __forceinline__ uint32_t finite2(uint32_t w) {  // with zeros in the place of what is not
   asm volatile("" : "+v"(w));
@@ -1017,7 +1015,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
       dma_seek(tile_at(d_it));
 #pragma unroll
       for (int x = 0; x < NS - 1; ++x) dma_step(x);
-      int slot = 0;
+      int slot = 0, into = NS - 1;
       for (int st = 0; st < steps; ++st) {
         if constexpr (NQ == 1)  // (a tile of one wave's own)
           asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -1026,8 +1024,9 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : NG == 4 ? 1 : NG == 2 || (D 
         uint32_t mask = ~0u;
         if constexpr (kMask) mask = static_cast<uint32_t>(__ballot(mload != 0.f));
         fetch_mask((st + 1) * NG + kg);
-        dma_step(slot == 0 ? NS - 1 : slot - 1);
+        dma_step(into);
         if (st * NG + kg < n) compute(tile_at(st * NG + kg) * kTile, (slot * NG + kg) * TILEB, 0, mask);
+        into = slot;
         slot = slot + 1 == NS ? 0 : slot + 1;
       }
     }

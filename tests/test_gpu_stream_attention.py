@@ -168,6 +168,14 @@ def test_window_attention_values_that_only_some_queries_see(dev, bad, sq, D):
     check(Fn.window_attention(q, k, v, 12, 1), ref, bound)
 
 
+@pytest.mark.parametrize("sq,D", [(3, 128), (40, 64), (200, 128)])
+def test_window_attention_largest_finite_values(dev, sq, D):
+    """Values next to the infinities are values."""
+    q, k, v = rnd(dev, 1, sq, 4, D), rnd(dev, 1, sq + 30, 2, D, seed=1), rnd(dev, 1, sq + 30, 2, D, seed=2)
+    v[:, 5, 0, 3], v[:, 29, 1, D - 1], v[:, 30 + sq // 2, 0, 17] = 2.0 ** 121, -(2.0 ** 127), torch.finfo(torch.bfloat16).max
+    check(Fn.window_attention(q, k, v, 12, 1), *window_ref(q, k, v, 12, 1))
+
+
 def test_window_attention_offsets_past_32_bits(dev):
     """Rows 64 KiB apart: the last keys lie 4.5 GB behind the first."""
     n, row = 70000, 32768
