@@ -1314,9 +1314,12 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     // Every row block turns the codes into values again, 32 rows 4 times as often as 128, but the fewer rows, the more
     // keys a step takes (4 tiles, 2 of 128 rows) and the fewer partial states leave the chip.  A step takes 2 us (32 rows,
     // 4 waves; 64 rows, 8 waves), 1.3 (128 rows, 8 waves).  us for 32 / 64 / 128 rows, head_dim 128: 49 tokens of 28/4
-    // heads over 300 slots 12.3 / 14.1 / 15.1, over 6000 32.6 / 24.1 / 27.3, 2 sequences of them 58.7 / 34.7 / 32.3;
-    // 169 tokens over 500 slots 13.5 / 19.6 / 20.9, over 2000 36.5 / 26.5 / 29.0, over 20000 375 / 115 / 86.
-    p.rb = steps_of(32, 4) <= 4 ? 32 : steps_of(64, 4) <= 8 ? 64 : 128;
+    // heads over 300 slots 11.6 / 13.1 / 14.1, over 6000 25.2 / 22.1 / 25.1, 2 sequences of them 42 / 29 / 30;
+    // 169 tokens over 500 slots 11.3 / 17.7 / 18.4, over 2000 27 / 23 / 26, over 20000 210 / 97 / 86.  64 rows as well
+    // where their blocks fill the chip without shares of the keys: 512 tokens of 32/8 heads over 4096 slots 90 / 58 / 64,
+    // of 64 43 / 41 / 46, 700 over 2000 37 / 29 / 43.
+    const int64_t blocks64 = heads * row_tiles(64);
+    p.rb = steps_of(32, 4) <= 4 ? 32 : steps_of(64, 4) <= 8 || (blocks64 >= cus * 7 / 8 && blocks64 <= per_cu * cus) ? 64 : 128;
     // Blocks of 128 rows that do not run at once: 4 waves, a tile a step (4096 tokens of 32/8 heads over 8192 slots 471
     // us, 516 with 8 waves; 1024 tokens, which do, 246 and 172).
     if (p.rb == 64 || (p.rb == 128 && heads * row_tiles(128) <= per_cu * cus)) p.waves = 8;
