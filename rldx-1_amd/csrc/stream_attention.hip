@@ -1325,10 +1325,10 @@ bool plan_of(Plan& p, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t 
     if (p.rb == 64 || (p.rb == 128 && heads * row_tiles(128) <= per_cu * cus)) p.waves = 8;
   } else {
     // The smallest row blocks whose workgroups run all at once, else 128 rows by 4 waves (us for 32 / 64 / 128 rows of 28/4
-    // heads of 128: 169 queries over 1449 keys 16 / 19 / 22, 640 x 640 26 / 16 / 22, 1280 x 1280, window 512, 50 / 32 / 28).
-    // But each block reads its keys again, and few blocks share them out: over long ranges 64 rows (169 x 3000 34 / 26 /
-    // 29), then 128 by 8 waves, two tiles a step (for 32 / 64 / these: 169 x 8192 78 / 47 / 36, 300 x 8192 147 / 106 / 57;
-    // 300 x 1449 29 / 21 / 25).  head_dim 64 with two workgroups of 32 rows on most CUs: 512 x 4096 of 32/8 heads 34 / 45 / 41.
+    // heads of 128: 169 queries over 1449 keys 14 / 19 / 22, 640 x 640, window 512, 23 / 16 / 21, 1280 x 1280 44 / 31 / 26).
+    // But each block reads its keys again, and few blocks share them out: over long ranges 64 rows, then 128 by 8 waves, two
+    // tiles a step (32 / 64 / these: 169 x 3000 25 / 26 / 26, 169 x 8192 54 / 46 / 35, 300 x 8192 104 / 103 / 56; 300 x 1449
+    // 25 / 20 / 25).  head_dim 64 with two workgroups of 32 rows on most CUs: 512 x 4096 of 32/8 heads 30 / 39 / 40.
     const int64_t blocks32 = heads * row_tiles(32), blocks64 = heads * row_tiles(64), steps32 = steps_of(32, 4);
     if (blocks32 <= per_cu * cus && (steps32 <= 16 || (blocks32 > cus && steps32 <= 64)))
       p.rb = 32;
